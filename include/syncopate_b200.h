@@ -39,6 +39,8 @@ extern "C" {
 #define SYN_ERR_RENDEZVOUS (-7)    /* peers did not show up at the rendezvous in time */
 #define SYN_ERR_UNSUPPORTED (-8)
 #define SYN_ERR_TOO_LARGE (-9)     /* more waves / ops / bytes than the fixed limits above */
+#define SYN_ERR_NO_PAGES (-10)     /* device: the free pages do not cover a step of the paged cache */
+#define SYN_ERR_BAD_INDEX (-11)    /* device: a length, page number or slot is out of range */
 
 const char* syn_strerror(int code);
 /* Text of the last CUDA error seen by this thread inside the library ("" if none). */
@@ -451,6 +453,123 @@ int syn_copy(const syn_attn_comm* comm, int num_sms, uint64_t signal_value, uint
 
 /* `comm` may be NULL (data already in place; flags, if any, raised by somebody else). */
 int syn_attention(const syn_attn_args* args, const syn_schedule* sched, const syn_attn_comm* comm, void* stream);
+
+/* ------------------------------------------------------------------ paged key-value cache
+ * Serving side of the attention operator: keys and values live in pages of `page_size` tokens
+ * (slot = page * page_size + offset), a request's pages are listed in its row of a block table, and
+ * every step of a batch is planned on the device, so that a step can be captured into a graph and
+ * replayed while the lengths grow.  None of the three calls allocates or synchronises.  All index
+ * tensors are int32 in device memory.  What a kernel finds out of range it neither reads nor writes;
+ * it records {code, request or token, value, block} in `status` (device int32[4], may be NULL) with
+ * code SYN_DEV_NO_PAGES (4) or SYN_DEV_BAD_INDEX (5), which syn_ctx_status maps to the codes above.
+ * `device` is the ordinal of the GPU that owns the tensors and `stream` (-1 = the current one).
+ */
+
+/* Plans one step of a batch.  Request z has lens[z] tokens in the cache and appends add[z] >= 0 more,
+ * or has ended (add[z] < 0).  The free pages are a stack, free_pages[0 .. *num_free).
+ *   1. The pages of ended requests, table[z][0 .. ceil(lens[z] / page_size)), are pushed onto the
+ *      stack, in request order.
+ *   2. Every other request gets ceil((lens + add) / page_size) - ceil(lens / page_size) pages from the
+ *      top of the stack, in request order, listed in its row of `table` behind those it has.
+ *   3. starts[z] = sum of the positive add[] before z, starts[requests] = their sum.  The i-th new
+ *      token of request z is token t = starts[z] + i of the step: positions[t] = lens[z] + i and
+ *      slots[t] = table[z][positions[t] / page_size] * page_size + positions[t] % page_size.
+ *      Behind the last token slots[t] = -1 and positions[t] = 0.
+ *   4. lens_out[z] = lens[z] + add[z], 0 for ended requests; *num_free_out = pages left.
+ * lens_out may be lens and num_free_out may be num_free (the state is then updated in place); apart
+ * from that no two arrays may overlap.  A step that does not fit (too few pages, rows or slots, or a
+ * length out of range) changes nothing: lens_out = lens, *num_free_out = *num_free, starts all 0,
+ * slots all -1, positions all 0, and `status` says why; free_pages beyond *num_free is scratch.
+ * At most SYN_PAGE_PLAN_MAX_REQUESTS requests, num_pages * page_size below 2^31. */
+#define SYN_PAGE_PLAN_MAX_REQUESTS 8192
+typedef struct syn_page_plan_args {
+  const int32_t* lens;     /* [requests] */
+  const int32_t* add;      /* [requests] */
+  int32_t* table;          /* [requests, width], rows table_stride elements apart */
+  int32_t* free_pages;     /* [num_pages] */
+  const int32_t* num_free; /* [1] */
+  int32_t* slots;          /* [tokens] */
+  int32_t* positions;      /* [tokens], may be NULL */
+  int32_t* starts;         /* [requests + 1] */
+  int32_t* lens_out;       /* [requests] */
+  int32_t* num_free_out;   /* [1] */
+  int32_t* status;
+  int64_t table_stride;
+  int32_t requests, width;
+  int32_t page_size, num_pages;
+  int32_t tokens;
+  int32_t device;
+} syn_page_plan_args;
+int syn_page_plan(const syn_page_plan_args* args, void* stream);
+
+/* Appends the keys and values of a step to the cache: row t of k and v [tokens, Hkv, D] goes to slot
+ * slots[t] of k_cache and v_cache [num_pages, page_size, Hkv, D] (one layout for both caches).  A
+ * negative slot is skipped; the slots of a call must differ from one another.  16-bit rows are copied;
+ * with cache_dtype SYN_CACHE_E4M3 the cache holds e4m3(x / scale[head]): the 32-bit quotient, limited to
+ * +-448 and rounded to the nearest, ties to even; NaN stays NaN.  D is a multiple of 16; base addresses
+ * and strides are multiples of 16 bytes. */
+#define SYN_CACHE_SAME 0 /* the type of q, k and v */
+#define SYN_CACHE_E4M3 1
+typedef struct syn_paged_append_args {
+  const void* k;
+  const void* v;
+  const int32_t* slots;
+  void* k_cache;
+  void* v_cache;
+  const float* k_scale; /* [Hkv], only with an 8-bit cache */
+  const float* v_scale;
+  int32_t* status;
+  int64_t k_strides[2]; /* elements: token, head */
+  int64_t v_strides[2];
+  int64_t cache_strides[3]; /* elements: page, slot, head */
+  int32_t tokens, Hkv, D;
+  int32_t page_size, num_pages;
+  int32_t dtype, cache_dtype;
+  int32_t device;
+} syn_paged_append_args;
+int syn_paged_append(const syn_paged_append_args* args, void* stream);
+
+/* Attention of the newest tokens of every request over its pages.  q and o [tokens, Hq, D], D 64, 128 or
+ * 256; request z owns the rows starts[z] .. starts[z + 1) (starts NULL: row z) and they are the last
+ * tokens of the lens[z] in its cache: row i of n sits at position p = lens[z] - n + i and sees the keys
+ * j <= p (`causal`; else all of them) with j > p - window (`window` > 0, causal only).
+ *   o = sum_j softmax_j(q . k_j * sm_scale) v_j,  lse [tokens, Hq] (may be NULL) = log2 sum_j exp(...)
+ * Keys and values of an 8-bit cache count as k_scale[head] and v_scale[head] times what is stored.  A row
+ * that sees no key gives 0 and lse = -inf; keys and values that a row does not see do not touch it,
+ * whatever they hold.  Rows outside all requests are left as they were.  A row that should see a key
+ * behind its row of the table, or on a page outside [0, num_pages), comes out as NaN (and in `status`).
+ * Base addresses and strides (in bytes) are multiples of 16.
+ * `workspace`: syn_paged_attention_workspace bytes, 16-byte aligned, any contents; it belongs to the call
+ * until the call has ended on the GPU. */
+typedef struct syn_paged_attn_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* table;  /* [requests, width], rows table_stride elements apart */
+  const int32_t* lens;   /* [requests] */
+  const int32_t* starts; /* [requests + 1] or NULL */
+  void* o;
+  float* lse;
+  const float* k_scale;
+  const float* v_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int64_t q_strides[2]; /* elements: token, head */
+  int64_t o_strides[2];
+  int64_t cache_strides[3]; /* elements: page, slot, head */
+  int64_t table_stride;
+  float sm_scale;
+  int32_t tokens, requests, Hq, Hkv, D;
+  int32_t page_size, num_pages, width;
+  int32_t causal, window;
+  int32_t dtype, cache_dtype;
+  int32_t num_sms; /* 0 = all */
+  int32_t device;
+} syn_paged_attn_args;
+int syn_paged_attention(const syn_paged_attn_args* args, void* stream);
+/* Bytes of workspace that every syn_paged_attention call on `num_sms` SMs can do with. */
+int64_t syn_paged_attention_workspace(int num_sms);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional, Sequence
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -17,6 +18,8 @@ SYN_MAX_WORLD = 8
 SYN_DTYPE_F16 = 0
 SYN_DTYPE_BF16 = 1
 SYN_ERR_TOO_LARGE = -9
+SYN_ERR_NO_PAGES = -10
+SYN_ERR_BAD_INDEX = -11
 
 ERRORS = {
     0: "SYN_OK",
@@ -29,6 +32,8 @@ ERRORS = {
     -7: "SYN_ERR_RENDEZVOUS",
     -8: "SYN_ERR_UNSUPPORTED",
     -9: "SYN_ERR_TOO_LARGE",
+    -10: "SYN_ERR_NO_PAGES",
+    -11: "SYN_ERR_BAD_INDEX",
 }
 
 
@@ -276,6 +281,127 @@ class AttnComm(C.Structure):
     ]
 
 
+SYN_CACHE_SAME = 0
+SYN_CACHE_E4M3 = 1
+PAGE_PLAN_MAX_REQUESTS = 8192
+
+
+class PagePlanArgs(C.Structure):
+    """``syn_page_plan_args``."""
+
+    _fields_ = [
+        ("lens", C.c_void_p),
+        ("add", C.c_void_p),
+        ("table", C.c_void_p),
+        ("free_pages", C.c_void_p),
+        ("num_free", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("lens_out", C.c_void_p),
+        ("num_free_out", C.c_void_p),
+        ("status", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("requests", C.c_int32),
+        ("width", C.c_int32),
+        ("page_size", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("tokens", C.c_int32),
+        ("device", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    """``syn_paged_append_args``; the strides are spelled out one by one (see :class:`Packer`)."""
+
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("status", C.c_void_p),
+        ("k_stride_token", C.c_int64),
+        ("k_stride_head", C.c_int64),
+        ("v_stride_token", C.c_int64),
+        ("v_stride_head", C.c_int64),
+        ("cache_stride_page", C.c_int64),
+        ("cache_stride_slot", C.c_int64),
+        ("cache_stride_head", C.c_int64),
+        ("tokens", C.c_int32),
+        ("Hkv", C.c_int32),
+        ("D", C.c_int32),
+        ("page_size", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("dtype", C.c_int32),
+        ("cache_dtype", C.c_int32),
+        ("device", C.c_int32),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    """``syn_paged_attn_args``; the strides are spelled out one by one (see :class:`Packer`)."""
+
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("o", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("status", C.c_void_p),
+        ("q_stride_token", C.c_int64),
+        ("q_stride_head", C.c_int64),
+        ("o_stride_token", C.c_int64),
+        ("o_stride_head", C.c_int64),
+        ("cache_stride_page", C.c_int64),
+        ("cache_stride_slot", C.c_int64),
+        ("cache_stride_head", C.c_int64),
+        ("table_stride", C.c_int64),
+        ("sm_scale", C.c_float),
+        ("tokens", C.c_int32),
+        ("requests", C.c_int32),
+        ("Hq", C.c_int32),
+        ("Hkv", C.c_int32),
+        ("D", C.c_int32),
+        ("page_size", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("width", C.c_int32),
+        ("causal", C.c_int32),
+        ("window", C.c_int32),
+        ("dtype", C.c_int32),
+        ("cache_dtype", C.c_int32),
+        ("num_sms", C.c_int32),
+        ("device", C.c_int32),
+    ]
+
+
+class Packer:
+    """Packs the fields of a flat ``Structure``, in order, into the bytes that its C struct has.  The
+    entry points of the paged cache take their arguments this way: a decode step calls them once a
+    layer, and filling 35 fields takes 0.5 us like this against 2 us through the ``Structure``."""
+
+    _CODES = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+
+    def __init__(self, cls):
+        fmt = struct.Struct("@" + "".join(self._CODES[t] for _, t in cls._fields_) + "0q")
+        if fmt.size != C.sizeof(cls):
+            raise AssertionError(f"{cls.__name__}: packed size {fmt.size}, C size {C.sizeof(cls)}")
+        self.pack = fmt.pack
+
+
+pack_page_plan = Packer(PagePlanArgs).pack
+pack_paged_append = Packer(PagedAppendArgs).pack
+pack_paged_attn = Packer(PagedAttnArgs).pack
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -341,6 +467,14 @@ def _declare(l: C.CDLL) -> None:
     l.syn_attention_plan.restype = C.c_int
     l.syn_attention_plan.argtypes = [C.POINTER(AttnArgs), C.POINTER(Schedule), C.c_void_p, C.c_void_p,
                                      C.POINTER(AttnPlan)]
+    l.syn_page_plan.restype = C.c_int
+    l.syn_page_plan.argtypes = [C.c_char_p, C.c_void_p]
+    l.syn_paged_append.restype = C.c_int
+    l.syn_paged_append.argtypes = [C.c_char_p, C.c_void_p]
+    l.syn_paged_attention.restype = C.c_int
+    l.syn_paged_attention.argtypes = [C.c_char_p, C.c_void_p]
+    l.syn_paged_attention_workspace.restype = C.c_int64
+    l.syn_paged_attention_workspace.argtypes = [C.c_int]
     l.syn_gemm_rs.restype = C.c_int
     l.syn_gemm_rs.argtypes = [C.POINTER(GemmRsArgs), C.POINTER(Schedule), C.POINTER(Schedule), C.c_void_p]
 

@@ -142,6 +142,8 @@ int status_to_err(int dev_code) {
     case 1: return SYN_ERR_TIMEOUT_FLAG;
     case 2: return SYN_ERR_TIMEOUT_MBAR;
     case 3: return SYN_ERR_TIMEOUT_COUNTER;
+    case 4: return SYN_ERR_NO_PAGES;
+    case 5: return SYN_ERR_BAD_INDEX;
     default: return SYN_ERR_INVALID;
   }
 }
@@ -162,6 +164,8 @@ const char* syn_strerror(int code) {
     case SYN_ERR_RENDEZVOUS: return "peer rendezvous timed out";
     case SYN_ERR_UNSUPPORTED: return "unsupported configuration";
     case SYN_ERR_TOO_LARGE: return "too many waves / ops / bytes for the fixed limits";
+    case SYN_ERR_NO_PAGES: return "not enough free pages for the step";
+    case SYN_ERR_BAD_INDEX: return "device: length, page number or slot out of range";
     default: return "unknown error";
   }
 }

@@ -45,6 +45,8 @@ int preload_copy_kernels();
 int preload_fused_kernels();
 int preload_gemm_kernels();
 int preload_attn_kernels();
+int preload_paged_kernels();
+int preload_paged_attn_kernels();
 
 // Maps a device status code (ptx.cuh) to the negative C-ABI code.
 int status_to_err(int dev_code);

@@ -19,6 +19,8 @@ enum : int {
   SYN_DEV_TIMEOUT_FLAG = 1,    // cross-GPU (or host-set) signal flag never reached its value
   SYN_DEV_TIMEOUT_MBAR = 2,    // intra-CTA mbarrier wait ran out (a pipeline bug)
   SYN_DEV_TIMEOUT_COUNTER = 3, // grid-wide counter never reached its value
+  SYN_DEV_NO_PAGES = 4,        // the free pages do not cover a step of the paged cache
+  SYN_DEV_BAD_INDEX = 5,       // a length, page number or slot out of range
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -117,6 +117,8 @@ int syn_preload(void) {
   if (rc == SYN_OK) rc = preload_fused_kernels();
   if (rc == SYN_OK) rc = preload_gemm_kernels();
   if (rc == SYN_OK) rc = preload_attn_kernels();
+  if (rc == SYN_OK) rc = preload_paged_kernels();
+  if (rc == SYN_OK) rc = preload_paged_attn_kernels();
   if (rc == SYN_OK) SYN_CUDA_TRY(cudaDeviceSynchronize());
   return rc;
 }

@@ -24,6 +24,7 @@ from .communication.common_descriptors import (
 )
 from .computation.gemm import ag_gemm, gemm, gemm_rs
 from .computation.gemm.plan import rs_remote_signals, rs_transport_program
+from .computation.paged import HEAD_DIMS, page_plan, paged_append, paged_attention
 from .interface import lower_comm_plan_to_raw_schedules
 from .runtime import SymmetricContext
 
@@ -852,3 +853,85 @@ class ContextParallelAttention:
         if self.sync_after and self.world > 1 and comm is not None:
             self.ctx.barrier(stream)
         return out
+
+
+class PagedKVCache:
+    """Key-value cache of a running batch: pages of ``page_size`` tokens that its requests share, one pool
+    of keys and values a layer, one block table for all layers.  The cache holds one rank's key-value
+    heads: nothing here talks to a peer.
+
+    A step is ``plan(add)`` once, then ``append`` and ``attend`` for every layer, all in the order of one
+    stream.  The buffers are made here and keep their addresses, so a step can be captured into a CUDA graph
+    and replayed; the lengths live on the device and grow with every replay.
+
+    A request is a row ``0 .. max_requests - 1``.  The tokens of a step lie behind one another, request by
+    request, at rows ``starts[z]:starts[z + 1]``; ``positions`` are their positions in their sequences.
+    ``cache_dtype=torch.float8_e4m3fn`` keeps 8 bits an element, scaled by ``k_scale`` / ``v_scale``
+    ``[layers, kv_heads]`` (float32).
+    """
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_requests: int, max_len: int,
+                 max_tokens: int, *, layers: int = 1, dtype: torch.dtype = torch.bfloat16,
+                 cache_dtype: Optional[torch.dtype] = None, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None, device=None):
+        if min(num_pages, page_size, kv_heads, head_dim, max_requests, max_len, max_tokens, layers) <= 0:
+            raise ValueError("the sizes of a cache must be positive")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
+        kept = cache_dtype or dtype
+        if kept not in (dtype, torch.float8_e4m3fn):
+            raise ValueError(f"a cache for {dtype} keeps {dtype} or torch.float8_e4m3fn, not {kept}")
+        scaled = kept is torch.float8_e4m3fn
+        if scaled != (k_scale is not None) or scaled != (v_scale is not None):
+            raise ValueError("k_scale and v_scale belong to an 8-bit cache, which needs both")
+        for s in (k_scale, v_scale):
+            if s is not None and tuple(s.shape) != (layers, kv_heads):
+                raise ValueError(f"scales must be [layers, kv_heads] = [{layers}, {kv_heads}]")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.page_size, self.dtype, self.device = page_size, dtype, device
+        ints = dict(dtype=torch.int32, device=device)
+        self.kv = torch.empty(layers, 2, num_pages, page_size, kv_heads, head_dim, dtype=kept, device=device)
+        self.k_scale = [None] * layers if k_scale is None else list(k_scale.to(device, torch.float32).contiguous())
+        self.v_scale = [None] * layers if v_scale is None else list(v_scale.to(device, torch.float32).contiguous())
+        self._k = [self.kv[i, 0] for i in range(layers)]
+        self._v = [self.kv[i, 1] for i in range(layers)]
+        self.table = torch.zeros(max_requests, -(-max_len // page_size), **ints)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, **ints)  # page 0 is on top
+        self.num_free = torch.full((1,), num_pages, **ints)
+        self.lens = torch.zeros(max_requests, **ints)
+        self.slots = torch.full((max_tokens,), -1, **ints)
+        self.positions = torch.zeros(max_tokens, **ints)
+        self.starts = torch.zeros(max_requests + 1, **ints)
+        self.status = torch.zeros(4, **ints)
+
+    def plan(self, add: torch.Tensor, stream=None) -> None:
+        """Plans a step in which request ``z`` appends ``add[z]`` tokens (int32 on the device); -1 ends the
+        request and gives its pages back.  A step that does not fit changes nothing and appends nothing:
+        see :meth:`check`."""
+        page_plan(self.lens, add, self.table, self.free_pages, self.num_free, self.page_size, self.slots, self.positions,
+                  self.starts, status=self.status, stream=stream)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0, stream=None) -> None:
+        """Writes the step's keys and values ``[tokens, kv_heads, head_dim]``.  Rows behind the step's last
+        token are padding and are not written."""
+        paged_append(k, v, self.slots, self._k[layer], self._v[layer], k_scale=self.k_scale[layer],
+                     v_scale=self.v_scale[layer], status=self.status, stream=stream)
+
+    def attend(self, q: torch.Tensor, layer: int = 0, *, sm_scale: Optional[float] = None, window: int = 0,
+               out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """Attention of the step's tokens ``q`` ``[tokens, q_heads, head_dim]`` over their sequences (see
+        ``paged_attention``).  Rows behind the step's last token are left as they were."""
+        return paged_attention(q, self._k[layer], self._v[layer], self.table, self.lens,
+                               q.shape[-1] ** -0.5 if sm_scale is None else sm_scale, starts=self.starts, window=window,
+                               k_scale=self.k_scale[layer], v_scale=self.v_scale[layer], out=out, lse=lse,
+                               status=self.status, stream=stream)
+
+    def check(self) -> None:
+        """Synchronises the device and raises ``SynError`` if a step since the last check did not fit
+        (``SYN_ERR_NO_PAGES``) or a length, page or slot was out of range (``SYN_ERR_BAD_INDEX``)."""
+        torch.cuda.synchronize(self.device)
+        words = self.status.tolist()
+        if words[0] != 0:
+            self.status.zero_()
+            code = {4: _L.SYN_ERR_NO_PAGES, 5: _L.SYN_ERR_BAD_INDEX}.get(words[0], -1)
+            raise _L.SynError(code, "paged cache", f"request={words[1]} value={words[2]} block={words[3]}")

@@ -182,7 +182,7 @@ class EmulatedContext:
         words = self.status.tolist()
         if words[0] != 0:
             self.status.zero_()
-            code = {1: -4, 2: -5, 3: -6}.get(words[0], -1)
+            code = {1: -4, 2: -5, 3: -6, 4: -10, 5: -11}.get(words[0], -1)
             raise L.SynError(code, "device status", f"wave={words[1]} flag={words[2]} block={words[3]}")
 
     def close(self) -> None:
