@@ -1,101 +1,97 @@
-// Attention of the newest tokens over a paged key-value cache.
-#include <math_constants.h>
+// Host side of the paged attention (see paged_attn_sm100.cuh).
+#include "paged_attn_sm100.cuh"
 
-#include "paged.cuh"
+#include <atomic>
 
 namespace syn {
 
-constexpr int PAGED_WARPS = 4;
+constexpr int PA_MAX_BLOCKS = 2;          // resident blocks an SM, over all variants
+constexpr int PA_MAX_UNIT = 32 * 128;     // rows x D of a unit, over all variants
+constexpr int PA_MAX_ROWS = 32;
 
-template <typename T>
-__device__ __forceinline__ float load16(const T* p);
-template <>
-__device__ __forceinline__ float load16(const __half* p) { return __half2float(*p); }
-template <>
-__device__ __forceinline__ float load16(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-template <>
-__device__ __forceinline__ float load16(const __nv_fp8_e4m3* p) { return static_cast<float>(*p); }
-
-// One block per new token and query head; its warps take the keys in turn and join at the end.
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(PAGED_WARPS * 32) paged_attn_kernel(syn_paged_attn_args p) {
-  constexpr int N = D / 32;
-  __shared__ float s_m[PAGED_WARPS], s_l[PAGED_WARPS], s_o[PAGED_WARPS][D];
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int z = t, first_row = t, rows = 1;
-  if (p.starts != nullptr) {
-    int a = 0, b = p.requests;  // the last request that starts at or before the token and has rows
-    while (b - a > 1) {
-      const int m = (a + b) >> 1;
-      (p.starts[m] <= t ? a : b) = m;
-    }
-    z = a;
-    first_row = p.starts[z];
-    rows = p.starts[z + 1] - first_row;
-    if (t < first_row || t >= first_row + rows) return;
-  }
-  const int64_t room = static_cast<int64_t>(p.width) * p.page_size;
-  int len = p.lens[z];
-  if (len < 0) {
-    if (threadIdx.x == 0) paged_record(p.status, SYN_DEV_BAD_INDEX, z, len);
-    len = 0;
-  }
-  if (len > room) len = static_cast<int>(min(room + 1, static_cast<int64_t>(INT_MAX)));
-  const int pos = len - rows + (t - first_row);
-  const int hi = p.causal ? min(len, pos + 1) : len;
-  const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  const int kh = h / (p.Hq / p.Hkv);
-  const float ks = p.k_scale ? p.k_scale[kh] : 1.f, vs = p.v_scale ? p.v_scale[kh] : 1.f;
-  const float mult = p.sm_scale * CUDART_L2E_F * ks;
-  float q[N], o[N] = {}, m = -CUDART_INF_F, l = 0.f;
-  const T* qp = static_cast<const T*>(p.q) + t * p.q_strides[0] + h * p.q_strides[1];
-  for (int i = 0; i < N; ++i) q[i] = load16(qp + i * 32 + lane);
-  for (int j = lo + warp; j < hi; j += PAGED_WARPS) {
-    const int page = j / p.page_size < p.width ? p.table[z * p.table_stride + j / p.page_size] : -1;
-    const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages);
-    if (!ok && lane == 0) paged_record(p.status, SYN_DEV_BAD_INDEX, z, page);
-    const int64_t at = ok ? page * p.cache_strides[0] + j % p.page_size * p.cache_strides[1] + kh * p.cache_strides[2] : 0;
-    float s = 0.f;
-    for (int i = 0; i < N; ++i) s += q[i] * load16(static_cast<const C*>(p.k_cache) + at + i * 32 + lane);
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-    s = ok ? s * mult : CUDART_NAN_F;
-    const float top = fmaxf(m, s), base = top == -CUDART_INF_F ? 0.f : top;
-    const float a = exp2f(m - base), w = exp2f(s - base);
-    l = l * a + w;
-    for (int i = 0; i < N; ++i) o[i] = o[i] * a + w * load16(static_cast<const C*>(p.v_cache) + at + i * 32 + lane);
-    m = top;
-  }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-  for (int i = 0; i < N; ++i) s_o[warp][i * 32 + lane] = o[i];
-  __syncthreads();
-  float top = -CUDART_INF_F, total = 0.f;
-  for (int w = 0; w < PAGED_WARPS; ++w) top = fmaxf(top, s_m[w]);
-  const float base = top == -CUDART_INF_F ? 0.f : top;
-  for (int w = 0; w < PAGED_WARPS; ++w) total += s_l[w] * exp2f(s_m[w] - base);
-  T* op = static_cast<T*>(p.o) + t * p.o_strides[0] + h * p.o_strides[1];
-  for (int d = threadIdx.x; d < D; d += PAGED_WARPS * 32) {
-    float x = 0.f;
-    for (int w = 0; w < PAGED_WARPS; ++w) x += s_o[w][d] * exp2f(s_m[w] - base);
-    op[d] = static_cast<T>(total == 0.f ? 0.f : x / total * vs);
-  }
-  if (threadIdx.x == 0 && p.lse != nullptr) p.lse[static_cast<int64_t>(t) * p.Hq + h] = top + log2f(total);
+static int64_t paged_workspace(int sms) {
+  const int64_t grid = static_cast<int64_t>(sms) * PA_MAX_BLOCKS;
+  return grid * PA_DESC * 4 + 2 * grid * (PA_MAX_ROWS * 2 + PA_MAX_UNIT) * 4;
 }
 
-template <typename T, typename C>
-static int launch_paged(const syn_paged_attn_args& a, cudaStream_t stream) {
-  const dim3 grid(a.tokens, a.Hq);
-  if (a.D == 64) paged_attn_kernel<T, C, 64><<<grid, PAGED_WARPS * 32, 0, stream>>>(a);
-  else if (a.D == 128) paged_attn_kernel<T, C, 128><<<grid, PAGED_WARPS * 32, 0, stream>>>(a);
-  else paged_attn_kernel<T, C, 256><<<grid, PAGED_WARPS * 32, 0, stream>>>(a);
-  SYN_CUDA_TRY(cudaGetLastError());
+// Opts the kernel into its shared memory, once a device.
+template <typename C>
+static int configure_paged() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  SYN_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return SYN_OK;
+  SYN_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  cudaFuncAttributes attr;
+  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_join_kernel<C>));
+  done.fetch_or(bit, std::memory_order_relaxed);
   return SYN_OK;
 }
 
-int preload_paged_attn_kernels() { return SYN_OK; }
+template <typename C>
+static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stream) {
+  int rc = configure_paged<C>();
+  if (rc != SYN_OK) return rc;
+  PagedAttnParams p;
+  p.a = a;
+  p.grid = sms * C::BLOCKS;
+  p.min_tiles = 4;
+  p.desc = static_cast<int32_t*>(a.workspace);
+  p.part_ml = reinterpret_cast<float*>(p.desc + p.grid * PA_DESC);
+  p.part_o = p.part_ml + static_cast<int64_t>(2) * p.grid * C::ROWS * 2;
+  paged_attn_kernel<C><<<p.grid, PA_THREADS, C::SMEM, stream>>>(p);
+  SYN_CUDA_TRY(cudaGetLastError());
+  if (p.grid < 2) return SYN_OK;
+  // The join's blocks are brought in while the last shares are still at work and wait for them there.
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(p.grid - 1);
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  SYN_CUDA_TRY(cudaLaunchKernelEx(&config, paged_join_kernel<C>, p));
+  return SYN_OK;
+}
+
+template <typename T, bool E4M3>
+static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stream) {
+  // Units of 32 rows where requests bring more than 16 rows a head on average.
+  const int64_t rows = static_cast<int64_t>(a.tokens) * (a.Hq / a.Hkv);
+  const bool two = rows > 16 * static_cast<int64_t>(a.requests);
+  if (a.D == 256) return launch_paged<PagedCfg<T, E4M3, 256, 1>>(a, sms, stream);
+  if (a.D == 128) {
+    return two ? launch_paged<PagedCfg<T, E4M3, 128, 2>>(a, sms, stream) : launch_paged<PagedCfg<T, E4M3, 128, 1>>(a, sms, stream);
+  }
+  return two ? launch_paged<PagedCfg<T, E4M3, 64, 2>>(a, sms, stream) : launch_paged<PagedCfg<T, E4M3, 64, 1>>(a, sms, stream);
+}
+
+template <typename T, bool E4M3>
+static int preload_paged() {
+  int rc = configure_paged<PagedCfg<T, E4M3, 64, 1>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 64, 2>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 128, 1>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 128, 2>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 256, 1>>();
+  return rc;
+}
+
+int preload_paged_attn_kernels() {
+  int rc = preload_paged<__half, false>();
+  if (rc == SYN_OK) rc = preload_paged<__half, true>();
+  if (rc == SYN_OK) rc = preload_paged<__nv_bfloat16, false>();
+  if (rc == SYN_OK) rc = preload_paged<__nv_bfloat16, true>();
+  return rc;
+}
 
 }  // namespace syn
 
-extern "C" int64_t syn_paged_attention_workspace(int num_sms) { return num_sms < 0 ? SYN_ERR_INVALID : 0; }
+extern "C" int64_t syn_paged_attention_workspace(int num_sms) {
+  return num_sms <= 0 ? SYN_ERR_INVALID : syn::paged_workspace(num_sms);
+}
 
 extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
   using namespace syn;
@@ -123,9 +119,14 @@ extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
     return SYN_ERR_INVALID;
   PagedDevice device(a->device);
   SYN_CUDA_TRY(device.error());
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != SYN_OK) return rc;
+  if (a->num_sms > 0 && a->num_sms < sms) sms = a->num_sms;
+  if (a->workspace == nullptr || a->workspace_bytes < paged_workspace(sms)) return SYN_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == SYN_DTYPE_BF16) {
-    return e4m3 ? launch_paged<__nv_bfloat16, __nv_fp8_e4m3>(p, s) : launch_paged<__nv_bfloat16, __nv_bfloat16>(p, s);
+    return e4m3 ? launch_paged<__nv_bfloat16, true>(p, sms, s) : launch_paged<__nv_bfloat16, false>(p, sms, s);
   }
-  return e4m3 ? launch_paged<__half, __nv_fp8_e4m3>(p, s) : launch_paged<__half, __half>(p, s);
+  return e4m3 ? launch_paged<__half, true>(p, sms, s) : launch_paged<__half, false>(p, sms, s);
 }

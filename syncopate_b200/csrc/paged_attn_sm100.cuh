@@ -1,0 +1,828 @@
+// Attention of the newest tokens over a paged key-value cache (decoding, drafted tokens).
+//
+// Mathematics.  Rows are (new token, query head) pairs.  Over its keys in any order a row keeps the
+// running maximum m of its scores (times log2 e), the sum l of 2^(s - m) and the output o = sum 2^(s - m) v,
+// rescaled by 2^(m - m') when the maximum rises; parts of a row's keys are joined by the same rule.
+//
+// What bounds it.  Every key and value is read once and serves the group of query heads that share it:
+// 4 * group * D operations for 2 * D stored numbers, about `group` operations a byte, against 250 at
+// which the matrix units would become the bound.  So the work is a stream from HBM, the matrix products
+// are small ones (16 rows, padded) on mma.sync, whose fragments stay in registers, and the layout is
+// chosen for loads in flight:
+//   * Every warp streams keys of its own through a ring of its own in shared memory (cp.async of 16
+//     bytes, a page lookup per key), so no barrier stands between loading and computing; the warps of a
+//     block meet only when a unit of rows ends.
+//   * The work (requests x key-value heads x row tiles x key tiles) is laid out in one line and cut into
+//     equal shares for a grid that fills the GPU, whatever the lengths; loads run on across the borders of
+//     units.  A unit that a border cuts leaves partial results, which a second small kernel joins in a fixed
+//     order: results do not depend on timing, there are no atomics and no state between calls.
+#pragma once
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace syn {
+
+constexpr int PA_WARPS = 4;
+constexpr int PA_THREADS = PA_WARPS * 32;
+constexpr int PA_DESC = 8;  // int32 words a block leaves for the join
+
+struct PagedAttnParams {
+  syn_paged_attn_args a;
+  int32_t grid;       // blocks of the launch
+  int32_t min_tiles;  // fewest key tiles worth a block
+  float* part_o;      // [2 * grid][rows of a unit][D]
+  float* part_ml;     // [2 * grid][rows of a unit][2]
+  int32_t* desc;      // [grid][PA_DESC]
+};
+
+template <typename T, bool E4M3_, int D_, int MT_>
+struct PagedCfg {
+  using type = T;
+  static constexpr bool E4M3 = E4M3_;
+  static constexpr int D = D_;
+  static constexpr int MT = MT_;                     // 16-row tiles of a unit
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int KEYS = E4M3 ? 32 : 16;        // keys of a warp's step
+  static constexpr int TILE = KEYS * PA_WARPS;       // keys of a block's step
+  static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
+  static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
+  static constexpr int STEPB = 2 * KEYS * ROWB;      // keys, then values
+  static constexpr int STAGES = D == 64 ? 4 : D == 128 && MT == 2 ? 2 : 3;
+  static constexpr int RING = STAGES * STEPB;        // bytes a warp
+  static constexpr bool QREG = MT == 1 && D <= 128;  // query fragments in registers, else in shared memory
+  static constexpr int KSTEPS = D / 16;
+  static constexpr int NT = D / 8;                   // 8-wide output tiles
+  static constexpr int DC = MT == 1 ? 32 : 16;       // output columns of a merge pass
+  static constexpr int NT_PASS = DC / 8;
+  static constexpr int PASSES = D / DC;
+  static constexpr int MERGE_LD = DC + 4;
+  static constexpr int SMEM_Q = QREG ? 0 : KSTEPS * MT * 512;
+  static constexpr int SMEM_MERGE = PA_WARPS * ROWS * MERGE_LD * 4;
+  static constexpr int SMEM_ML = PA_WARPS * ROWS * 2 * 4;
+  static constexpr int SMEM = PA_WARPS * RING + SMEM_Q + SMEM_MERGE + SMEM_ML;
+  static constexpr int BLOCKS = (227 * 1024) / (SMEM + 1024) >= 2 ? 2 : 1;  // resident on an SM
+};
+
+// ----------------------------------------------------------------------------- instructions
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two e4m3 bytes as two halves (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t x) {
+  uint32_t y;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (BF16) {
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  }
+}
+
+// ----------------------------------------------------------------------------- the line of work
+struct PagedRequest {
+  int s0, n;       // rows of q: first one, how many
+  int len;         // keys (one more than the table has room for, where the length says more)
+  int first;       // first key that any row sees
+  int tiles, rt;   // key tiles of a unit; row tiles a head
+};
+
+template <typename C>
+__device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args& a, int z) {
+  PagedRequest r;
+  r.s0 = z, r.n = 1;
+  if (a.starts != nullptr) {
+    r.s0 = min(max(a.starts[z], 0), a.tokens);
+    r.n = min(max(a.starts[z + 1], r.s0), a.tokens) - r.s0;
+  }
+  const long long room = static_cast<long long>(a.width) * a.page_size;
+  int len = max(a.lens[z], 0);
+  if (len > room) len = static_cast<int>(min(room + 1, static_cast<long long>(INT_MAX)));
+  r.len = len;
+  r.first = a.window > 0 ? max(0, min(len, len - r.n - a.window + 1)) : 0;
+  r.tiles = max(1, (len - r.first + C::TILE - 1) / C::TILE);
+  r.rt = (r.n * (a.Hq / a.Hkv) + C::ROWS - 1) / C::ROWS;
+  return r;
+}
+
+__device__ __forceinline__ long long paged_border(long long total, int shares, int c) { return total * c / shares; }
+
+// Position on the line: key tile `tile` of unit `sub` (head * row tiles + row tile) of request z.
+template <typename C>
+struct PagedCursor {
+  int z, sub, tile;
+  PagedRequest r;
+
+  __device__ __forceinline__ void at(const syn_paged_attn_args& a, int z_, long long rest) {
+    z = z_;
+    r = paged_request<C>(a, z);
+    sub = static_cast<int>(rest / r.tiles);
+    tile = static_cast<int>(rest % r.tiles);
+  }
+  // To the first tile of the next unit; the caller knows that there is one.
+  __device__ __forceinline__ void next_unit(const syn_paged_attn_args& a) {
+    tile = 0;
+    if (++sub < a.Hkv * r.rt) return;
+    sub = 0;
+    do {
+      ++z;
+      r = paged_request<C>(a, z);
+    } while (r.rt == 0 && z + 1 < a.requests);
+  }
+};
+
+// ----------------------------------------------------------------------------- fragments
+// Calls f(nt, b0, b1) with the fragments of 16 keys (group `kk` of the step) for every 8-wide output tile.
+// Output tile nt holds, in its column c, dimension 8 nt + c of 16-bit values.  8-bit values are fetched 16
+// (D = 64: 8) dimensions of one key at a time and paired with the next key's, so there column c of tile nt is
+// dimension 16 c + nt % 16 + 128 (nt / 16) (D = 64: 8 c + nt): a permutation that the epilogue undoes.
+template <typename C, typename F>
+__device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
+  if constexpr (!C::E4M3) {
+    const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+    for (int j = 0; j < C::D / 16; ++j) {
+      uint32_t b[4];
+      ldsm4t(v + row * C::ROWB + (((j * 2 + (lane >> 4)) ^ (row & 7)) << 4), b);
+      f(2 * j, b[0], b[1]);
+      f(2 * j + 1, b[2], b[3]);
+    }
+  } else {
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t row0 = v + (kk * 16 + 2 * t) * C::ROWB;
+    auto words = [&](int nt, uint32_t x0, uint32_t x1, uint32_t x8, uint32_t x9) {
+      const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);
+      const uint32_t lo89 = __byte_perm(x8, x9, 0x5140), hi89 = __byte_perm(x8, x9, 0x7362);
+      f(nt, e4m3x2_to_h2(lo01), e4m3x2_to_h2(lo89));
+      f(nt + 1, e4m3x2_to_h2(lo01 >> 16), e4m3x2_to_h2(lo89 >> 16));
+      f(nt + 2, e4m3x2_to_h2(hi01), e4m3x2_to_h2(hi89));
+      f(nt + 3, e4m3x2_to_h2(hi01 >> 16), e4m3x2_to_h2(hi89 >> 16));
+    };
+    if constexpr (C::D == 64) {
+      const uint32_t at = (((g >> 1) ^ t) << 4) + (g & 1) * 8;
+      const uint2 x0 = lds8(row0 + at), x1 = lds8(row0 + C::ROWB + at);
+      const uint2 x8 = lds8(row0 + 8 * C::ROWB + at), x9 = lds8(row0 + 9 * C::ROWB + at);
+      words(0, x0.x, x1.x, x8.x, x9.x);
+      words(4, x0.y, x1.y, x8.y, x9.y);
+    } else {
+#pragma unroll
+      for (int half = 0; half < C::D / 128; ++half) {
+        const uint32_t at = ((g + half * 8) ^ (t << 1)) << 4;
+        const uint4 x0 = lds16(row0 + at), x1 = lds16(row0 + C::ROWB + at);
+        const uint4 x8 = lds16(row0 + 8 * C::ROWB + at), x9 = lds16(row0 + 9 * C::ROWB + at);
+        words(half * 16, x0.x, x1.x, x8.x, x9.x);
+        words(half * 16 + 4, x0.y, x1.y, x8.y, x9.y);
+        words(half * 16 + 8, x0.z, x1.z, x8.z, x9.z);
+        words(half * 16 + 12, x0.w, x1.w, x8.w, x9.w);
+      }
+    }
+  }
+}
+
+// Place of 16-byte chunk `chunk` of row `row` in a warp's ring (chosen so that the reads above and those of
+// the keys below meet no bank twice; D = 64 in 8 bits reads its values two deep).
+template <typename C, bool VALUES>
+__device__ __forceinline__ uint32_t ring_at(int row, int chunk) {
+  int c = chunk;
+  if constexpr (!C::E4M3) c ^= row & 7;
+  else if constexpr (VALUES) c ^= C::D == 64 ? (row >> 1) & 3 : ((row >> 1) & 3) << 1;
+  else if constexpr (C::D != 64) c ^= (row & 1) << 2;
+  return row * C::ROWB + (c << 4);
+}
+
+// Dimension of entry e (0 .. DC - 1) of merge pass `pass`; entries 2 i and 2 i + 1 are neighbours.
+template <typename C>
+__device__ __forceinline__ int merge_dim(int pass, int e) {
+  if constexpr (!C::E4M3) return pass * C::DC + e;
+  const int nt = pass * C::NT_PASS + e % C::NT_PASS, c = e / C::NT_PASS;
+  if constexpr (C::D == 64) return 8 * c + nt;
+  return (nt / 16) * 128 + 16 * c + nt % 16;
+}
+// Entry of column c of the pass's i-th output tile.
+template <typename C>
+__device__ __forceinline__ int merge_entry(int i, int c) {
+  return C::E4M3 ? c * C::NT_PASS + i : i * 8 + c;
+}
+
+template <typename C>
+__global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+  using T = typename C::type;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool MBF16 = BF16 && !C::E4M3;  // type of the matrix products: 8-bit values are halves there
+  constexpr int MT = C::MT;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long s_sum[PA_WARPS];
+  __shared__ long long s_rest;
+  __shared__ int s_z;
+  const syn_paged_attn_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int group = a.Hq / a.Hkv;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this block's share of the line
+  const int per = (a.requests + PA_THREADS - 1) / PA_THREADS;
+  const int z0 = min(tid * per, a.requests), z1 = min(z0 + per, a.requests);
+  long long mine = 0;
+  for (int z = z0; z < z1; ++z) {
+    const PagedRequest r = paged_request<C>(a, z);
+    mine += static_cast<long long>(r.tiles) * a.Hkv * r.rt;
+    if (blockIdx.x == 0) {
+      if (a.lens[z] < 0) paged_record(a.status, SYN_DEV_BAD_INDEX, z, a.lens[z]);
+      if (a.starts != nullptr && (a.starts[z] < 0 || a.starts[z + 1] < a.starts[z] || a.starts[z + 1] > a.tokens))
+        paged_record(a.status, SYN_DEV_BAD_INDEX, z, a.starts[z + 1]);
+    }
+  }
+  long long upto = mine;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(~0u, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) s_sum[warp] = upto;
+  __syncthreads();
+  long long total = 0;
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) upto += s_sum[w];
+    total += s_sum[w];
+  }
+  const int shares = static_cast<int>(min(static_cast<long long>(p.grid), max(1LL, total / p.min_tiles)));
+  const int block = blockIdx.x;
+  const long long t0 = block < shares ? paged_border(total, shares, block) : total;
+  const long long t1 = block < shares ? paged_border(total, shares, block + 1) : total;
+  if (t0 >= t1) {
+    if (tid < PA_DESC) p.desc[block * PA_DESC + tid] = 0;
+    return;
+  }
+  if (upto - mine <= t0 && t0 < upto) {
+    long long rest = t0 - (upto - mine);
+    int z = z0;
+    for (; z < z1; ++z) {
+      const PagedRequest r = paged_request<C>(a, z);
+      const long long w = static_cast<long long>(r.tiles) * a.Hkv * r.rt;
+      if (rest < w) break;
+      rest -= w;
+    }
+    s_z = z;
+    s_rest = rest;
+  }
+  __syncthreads();
+
+  PagedCursor<C> cur;
+  cur.at(a, s_z, s_rest);
+
+  // ---- producer: loads run STAGES - 1 steps ahead, across units
+  const uint32_t ring = smem_u32(smem) + warp * C::RING;
+  PagedCursor<C> ahead = cur;
+  long long t_ahead = t0;
+  int page = -2, inside = 0;  // page of this lane's key (-2: none), slot in it
+  int head_ahead = ahead.sub / max(ahead.r.rt, 1);
+  auto look_up = [&]() {
+    page = -2;
+    if (t_ahead < t1) {
+      const int key = ahead.r.first + ahead.tile * C::TILE + warp * C::KEYS + (lane & (C::KEYS - 1));
+      if (key < ahead.r.len) {
+        const int i = key / a.page_size;
+        inside = key - i * a.page_size;
+        page = i < a.width ? __ldg(a.table + ahead.z * a.table_stride + i) : -1;
+      }
+    }
+  };
+  auto issue = [&](int stage) {
+    if (t_ahead < t1) {
+      long long off = -2;
+      if (page != -2) {
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) {
+          off = page * a.cache_strides[0] + inside * a.cache_strides[1] + head_ahead * a.cache_strides[2];
+          if (C::E4M3 == false) off *= 2;
+        } else {
+          off = -1;
+          paged_record(a.status, SYN_DEV_BAD_INDEX, ahead.z, page);
+        }
+      }
+      const uint32_t slot = ring + stage * C::STEPB;
+#pragma unroll
+      for (int i = 0; i < C::KEYS * C::CPR / 32; ++i) {
+        const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
+        const long long o = __shfl_sync(~0u, off, row);
+        const uint32_t kd = slot + ring_at<C, false>(row, chunk), vd = slot + C::KEYS * C::ROWB + ring_at<C, true>(row, chunk);
+        if (o != -1) {
+          const long long at = o < 0 ? 0 : o + chunk * 16;
+          const uint32_t bytes = o < 0 ? 0 : 16;  // keys behind the end come as zeros
+          cp_async16(kd, static_cast<const char*>(a.k_cache) + at, bytes);
+          cp_async16(vd, static_cast<const char*>(a.v_cache) + at, bytes);
+        } else {  // no such page: NaN in every type
+          sts16(kd, ~0u, ~0u, ~0u, ~0u);
+          sts16(vd, ~0u, ~0u, ~0u, ~0u);
+        }
+      }
+      ++t_ahead;
+      if (++ahead.tile == ahead.r.tiles) {
+        if (t_ahead < t1) ahead.next_unit(a);
+        head_ahead = ahead.sub / ahead.r.rt;
+      }
+      look_up();
+    }
+    cp_async_commit();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+
+  const uint32_t q_smem = smem_u32(smem) + PA_WARPS * C::RING;
+  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * C::RING + C::SMEM_Q);
+  float* s_m = merge + C::SMEM_MERGE / 4;  // [warp][row]
+  float* s_l = s_m + PA_WARPS * C::ROWS;
+  int stage = 0;
+  long long t = t0;
+  int first_open = 0, first_mid = 0, parts = 0, tail_from_start = 0, tail_slot = 0;
+  const int z_first = cur.z, sub_first = cur.sub;
+  bool first_segment = true;
+
+  while (t < t1) {
+    // ---- a unit: rows row0 .. row0 + rows of head kv_head of request z
+    const PagedRequest r = cur.r;
+    const int kv_head = cur.sub / r.rt, row0 = (cur.sub - kv_head * r.rt) * C::ROWS;
+    const int rows = min(C::ROWS, r.n * group - row0);
+    const int pos0 = r.len - r.n;
+    const int tiles = static_cast<int>(min(static_cast<long long>(r.tiles - cur.tile), t1 - t));
+    int lo[2 * MT], hi[2 * MT];  // keys that rows g, g + 8, ... see
+    float mult[2 * MT];
+    const T* qrow[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int row = row0 + min(g + 8 * i, rows - 1);  // rows behind the last repeat it
+      const int tok = row / group, head = kv_head * group + row - tok * group;
+      hi[i] = a.causal ? min(r.len, pos0 + tok + 1) : r.len;
+      lo[i] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
+      mult[i] = a.sm_scale * CUDART_L2E_F;
+      qrow[i] = static_cast<const T*>(a.q) + static_cast<int64_t>(r.s0 + tok) * a.q_strides[0] + head * a.q_strides[1];
+    }
+    const int tok_a = row0 / group, tok_b = (row0 + rows - 1) / group;
+    const int all_lo = a.window > 0 ? max(0, pos0 + tok_b - a.window + 1) : 0;  // keys that every row sees
+    const int all_hi = a.causal ? min(r.len, pos0 + tok_a + 1) : r.len;
+
+    // ---- query fragments
+    if constexpr (C::E4M3) {
+      const float ks = a.k_scale[kv_head];
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) mult[i] *= ks;
+    }
+    float up[2 * MT];  // bf16 queries over 8-bit keys: a power of two brings each row into the range of halves
+    if constexpr (C::E4M3 && BF16) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) {
+        uint32_t top = 0;  // largest magnitude as bits
+#pragma unroll
+        for (int c = 0; c < C::D / 32; ++c) {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(qrow[i]) + c * 4 + t4);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
+        }
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+        const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
+        const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
+        up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+        mult[i] *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+      }
+    }
+    auto q_frag = [&](int ks, int mt, uint32_t (&f)[4]) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const T* q = qrow[2 * mt + half];
+        uint32_t x, y;
+        if constexpr (!C::E4M3) {
+          x = __ldg(reinterpret_cast<const uint32_t*>(q) + ks * 8 + t4);
+          y = __ldg(reinterpret_cast<const uint32_t*>(q) + ks * 8 + t4 + 4);
+        } else {  // the order in which the 8-bit keys are fetched
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + (t4 + ks / 4 * 4) * 4 + ks % 4);
+          x = v.x, y = v.y;
+          if constexpr (BF16) {
+            const float s = up[2 * mt + half];
+            const float2 xf = unpack2<true>(x), yf = unpack2<true>(y);
+            x = pack2<false>(xf.x * s, xf.y * s);
+            y = pack2<false>(yf.x * s, yf.y * s);
+          }
+        }
+        f[half] = x;
+        f[2 + half] = y;
+      }
+    };
+    uint32_t qreg[C::QREG ? C::KSTEPS : 1][4];
+    if constexpr (C::QREG) {
+#pragma unroll
+      for (int ks = 0; ks < C::KSTEPS; ++ks) q_frag(ks, 0, qreg[ks]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::KSTEPS * MT / PA_WARPS; ++i) {
+        const int f = i * PA_WARPS + warp;
+        uint32_t x[4];
+        if constexpr (MT == 1) {
+          q_frag(f, 0, x);
+        } else {
+          if (f % MT == 0) q_frag(f / MT, 0, x);
+          else q_frag(f / MT, MT - 1, x);
+        }
+        sts16(q_smem + f * 512 + lane * 16, x[0], x[1], x[2], x[3]);
+      }
+      __syncthreads();
+    }
+
+    float o[MT][C::NT][4], m[2 * MT], l[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) m[i] = -CUDART_INF_F, l[i] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[mt][nt][c] = 0.f;
+
+    for (int i = 0; i < tiles; ++i) {
+      cp_async_wait<C::STAGES - 2>();
+      __syncwarp();
+      issue(stage == 0 ? C::STAGES - 1 : stage - 1);  // into the slot read in the step before
+      const uint32_t k_at = ring + stage * C::STEPB, v_at = k_at + C::KEYS * C::ROWB;
+      if (++stage == C::STAGES) stage = 0;
+      const int base = r.first + (cur.tile + i) * C::TILE + warp * C::KEYS;
+      if (base >= r.len) continue;
+
+      // ---- scores
+      constexpr int SN = C::KEYS / 8;
+      float s[MT][SN][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[mt][n][c] = 0.f;
+      auto q_at = [&](int ks, int mt, uint32_t (&f)[4]) {
+        if constexpr (C::QREG) {
+          f[0] = qreg[ks][0], f[1] = qreg[ks][1], f[2] = qreg[ks][2], f[3] = qreg[ks][3];
+        } else {
+          const uint4 x = lds16(q_smem + (ks * MT + mt) * 512 + lane * 16);
+          f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+        }
+      };
+      if constexpr (!C::E4M3) {
+        const int row = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+        for (int ks = 0; ks < C::KSTEPS; ++ks) {
+          uint32_t b[4], f[4];
+          ldsm4(k_at + row * C::ROWB + (((ks * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), b);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            q_at(ks, mt, f);
+            mma16816<MBF16>(s[mt][0], f, b[0], b[1]);
+            mma16816<MBF16>(s[mt][1], f, b[2], b[3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int part = 0; part < C::D / 64; ++part) {
+          uint32_t f[4][MT][4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) q_at(part * 4 + w, mt, f[w][mt]);
+#pragma unroll
+          for (int n = 0; n < SN; ++n) {
+            const uint4 x = lds16(k_at + ring_at<C, false>(n * 8 + g, t4 + part * 4));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t b0 = e4m3x2_to_h2(w[j]), b1 = e4m3x2_to_h2(w[j] >> 16);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) mma16816<false>(s[mt][n], f[j][mt], b0, b1);
+            }
+          }
+        }
+      }
+
+      // ---- weights
+      const bool whole = base >= all_lo && base + C::KEYS <= all_hi;  // every row sees every key
+      float alpha[2 * MT];
+      bool rose = false;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int x = 2 * mt + half;
+          float top = m[x];
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& v = s[mt][n][2 * half + c];
+              v *= mult[x];
+              const int key = base + n * 8 + t4 * 2 + c;
+              if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
+              top = fmaxf(top, v);
+            }
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+          rose |= top > m[x];
+          const float zero = top == -CUDART_INF_F ? 0.f : top;
+          alpha[x] = ex2(m[x] - zero);
+          m[x] = top;
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& v = s[mt][n][2 * half + c];
+              v = ex2(v - zero);
+              sum += v;
+            }
+          l[x] = l[x] * alpha[x] + sum;
+        }
+      if (__any_sync(~0u, rose)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[mt][nt][c] *= alpha[2 * mt + c / 2];
+      }
+
+      // ---- values.  The weights enter the product as two 16-bit numbers, the second one what the first
+      // left, so that their rounding (2^-9 alone) does not add to that of the output.
+#pragma unroll
+      for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+        uint32_t ph[MT][4], pl[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float* v = &s[mt][2 * kk + (q >> 1)][2 * (q & 1)];
+            ph[mt][q] = pack2<MBF16>(v[0], v[1]);
+            const float2 b = unpack2<MBF16>(ph[mt][q]);
+            pl[mt][q] = pack2<MBF16>(v[0] - b.x, v[1] - b.y);
+          }
+        bool odd = false;  // values that are not finite, at keys that not every row sees
+        if (!whole && r.n > 1) {
+          constexpr uint32_t EXP = MBF16 ? 0x7F807F80u : 0x7C007C00u, ONE = MBF16 ? 0x00800080u : 0x04000400u;
+          each_v<C>(v_at, lane, kk, [&](int, uint32_t b0, uint32_t b1) {
+            odd |= ((((b0 & EXP) + ONE) | ((b1 & EXP) + ONE)) & 0x80008000u) != 0;
+          });
+          odd = __any_sync(~0u, odd);
+        }
+        if (!odd) {
+          each_v<C>(v_at, lane, kk, [&](int nt, uint32_t b0, uint32_t b1) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<MBF16>(o[mt][nt], ph[mt], b0, b1);
+              mma16816<MBF16>(o[mt][nt], pl[mt], b0, b1);
+            }
+          });
+        } else {
+          // Zero times infinity: such values may only enter the rows that see them, so one row at a time,
+          // with what it does not see taken out.
+#pragma unroll
+          for (int x = 0; x < 2 * MT; ++x) {
+            const int mt = x >> 1, half = x & 1;
+#pragma unroll 1
+            for (int row = 0; row < 8; ++row) {
+              const int row_lo = __shfl_sync(~0u, lo[x], row * 4), row_hi = __shfl_sync(~0u, hi[x], row * 4);
+              const int key = base + kk * 16 + t4 * 2;
+              auto seen = [&](int k) {
+                return (k >= row_lo && k < row_hi ? 0xFFFFu : 0u) | (k + 1 >= row_lo && k + 1 < row_hi ? 0xFFFF0000u : 0u);
+              };
+              const uint32_t mask0 = seen(key), mask1 = seen(key + 8);
+              each_v<C>(v_at, lane, kk, [&](int nt, uint32_t b0, uint32_t b1) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<MBF16>(c, ph[mt], b0 & mask0, b1 & mask1);
+                mma16816<MBF16>(c, pl[mt], b0 & mask0, b1 & mask1);
+                if (g == row) {
+                  o[mt][nt][2 * half] += c[2 * half];
+                  o[mt][nt][2 * half + 1] += c[2 * half + 1];
+                }
+              });
+            }
+          }
+        }
+      }
+    }
+
+    // ---- the warps' parts of the unit are put together
+#pragma unroll
+    for (int x = 0; x < 2 * MT; ++x) {
+      l[x] += __shfl_xor_sync(~0u, l[x], 1);
+      l[x] += __shfl_xor_sync(~0u, l[x], 2);
+      if (t4 == 0) s_m[warp * C::ROWS + g + 8 * x] = m[x], s_l[warp * C::ROWS + g + 8 * x] = l[x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2 * MT; ++x) {
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + g + 8 * x]);
+      const float f = ex2(m[x] - (top == -CUDART_INF_F ? 0.f : top));
+#pragma unroll
+      for (int nt = 0; nt < C::NT; ++nt) {
+        o[x >> 1][nt][2 * (x & 1)] *= f;
+        o[x >> 1][nt][2 * (x & 1) + 1] *= f;
+      }
+    }
+    constexpr int TPR = C::DC / 4;  // threads a row
+    const int row = tid / TPR, entry = (tid % TPR) * 4;
+    float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + row]);
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) sum += s_l[w * C::ROWS + row] * ex2(s_m[w * C::ROWS + row] - (top == -CUDART_INF_F ? 0.f : top));
+    const bool from_start = cur.tile == 0, to_end = cur.tile + tiles == r.tiles, partial = !(from_start && to_end);
+    const int part = 2 * block + (first_segment ? 0 : 1);
+    const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
+    float factor = 1.f;
+    if (!partial) {
+      factor = sum == 0.f ? 0.f : 1.f / sum;
+      if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
+    }
+    if (row < rows && entry == 0) {
+      if (partial) {
+        p.part_ml[(part * C::ROWS + row) * 2] = top;
+        p.part_ml[(part * C::ROWS + row) * 2 + 1] = sum;
+      } else if (a.lse != nullptr) {
+        a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+      }
+    }
+    T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+    float* out_part = p.part_o + (static_cast<int64_t>(part) * C::ROWS + row) * C::D;
+#pragma unroll
+    for (int pass = 0; pass < C::PASSES; ++pass) {
+      if (pass > 0) __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 2 * MT; ++x) {
+        if (g + 8 * x < rows) {
+          float* to = merge + (warp * C::ROWS + g + 8 * x) * C::MERGE_LD;
+#pragma unroll
+          for (int n = 0; n < C::NT_PASS; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              to[merge_entry<C>(n, t4 * 2 + c)] = o[x >> 1][pass * C::NT_PASS + n][2 * (x & 1) + c];
+        }
+      }
+      __syncthreads();
+      if (row < rows) {
+        float4 v = *reinterpret_cast<const float4*>(merge + row * C::MERGE_LD + entry);
+#pragma unroll
+        for (int w = 1; w < PA_WARPS; ++w) {
+          const float4 u = *reinterpret_cast<const float4*>(merge + (w * C::ROWS + row) * C::MERGE_LD + entry);
+          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        const int d0 = merge_dim<C>(pass, entry), d1 = merge_dim<C>(pass, entry + 2);
+        if (partial) {
+          *reinterpret_cast<float2*>(out_part + d0) = make_float2(v.x, v.y);
+          *reinterpret_cast<float2*>(out_part + d1) = make_float2(v.z, v.w);
+        } else {
+          *reinterpret_cast<uint32_t*>(out + d0) = pack2<BF16>(v.x * factor, v.y * factor);
+          *reinterpret_cast<uint32_t*>(out + d1) = pack2<BF16>(v.z * factor, v.w * factor);
+        }
+      }
+    }
+    __syncthreads();
+
+    // ---- what the join needs to know
+    if (first_segment) {
+      first_mid = !from_start;
+      first_open = !to_end;
+      if (first_mid) {  // the block that holds the unit's last tile
+        const long long end = t + (r.tiles - cur.tile);
+        int c = static_cast<int>(min((end * shares - 1) / total, static_cast<long long>(shares - 1)));
+        while (c + 1 < shares && paged_border(total, shares, c + 1) < end) ++c;
+        while (paged_border(total, shares, c) >= end) --c;
+        parts = c - block + 2;
+      }
+    }
+    if (from_start && !to_end) tail_from_start = 1, tail_slot = part;
+    first_segment = false;
+    t += tiles;
+    if (t < t1) cur.next_unit(a);
+  }
+  if (tid == 0) {
+    int32_t* d = p.desc + block * PA_DESC;
+    d[0] = first_mid;
+    d[1] = z_first;
+    d[2] = sub_first;
+    d[3] = parts;
+    d[4] = tail_from_start;
+    d[5] = tail_slot;
+    d[6] = first_open;
+    d[7] = 0;
+  }
+}
+
+// Joins the parts of the units that borders between blocks cut: block c takes the unit that the border
+// before block c + 1 cuts, if that is the first border in it.  A warp takes a row.
+template <typename C>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+  using T = typename C::type;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int N = C::D / 64;  // pairs of columns a lane
+  const syn_paged_attn_args& a = p.a;
+  const int c = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 d0 = *reinterpret_cast<const int4*>(p.desc + c * PA_DESC);
+  const int2 before = *reinterpret_cast<const int2*>(p.desc + (c - 1) * PA_DESC + 4);
+  if (!d0.x || !before.x) return;
+  const int z = d0.y, sub = d0.z, parts = d0.w;
+  const PagedRequest r = paged_request<C>(a, z);
+  const int group = a.Hq / a.Hkv, kv_head = sub / r.rt, row0 = (sub - kv_head * r.rt) * C::ROWS;
+  const int rows = min(C::ROWS, r.n * group - row0);
+  auto slot = [&](int i) { return i == 0 ? before.y : 2 * (c - 1 + i); };
+  for (int row = warp; row < rows; row += 8) {
+    float top = -CUDART_INF_F;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[(slot(i) * C::ROWS + row) * 2]);
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    const float zero = top == -CUDART_INF_F ? 0.f : top;
+    float sum = 0.f;
+    float2 v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const int64_t at = static_cast<int64_t>(slot(i)) * C::ROWS + row;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+      const float w = ex2(ml.x - zero);
+      sum += ml.y * w;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float2 u = *reinterpret_cast<const float2*>(p.part_o + at * C::D + j * 64 + lane * 2);
+        v[j].x += u.x * w, v[j].y += u.y * w;
+      }
+    }
+    float factor = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
+    const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
+    T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
+    if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+  }
+}
+
+}  // namespace syn
