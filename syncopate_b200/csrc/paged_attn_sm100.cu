@@ -5,7 +5,6 @@
 
 namespace syn {
 
-constexpr int PA_MAX_BLOCKS = 2;          // resident blocks an SM, over all variants
 constexpr int PA_MAX_UNIT = 32 * 128;     // rows x D of a unit, over all variants
 constexpr int PA_MAX_ROWS = 32;
 
@@ -49,7 +48,7 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.grid - 1);
-  config.blockDim = dim3(256);
+  config.blockDim = dim3(PA_JOIN_WARPS * 32);
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;
@@ -59,23 +58,33 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
 
 template <typename T, bool E4M3>
 static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stream) {
-  // Units of 32 rows where requests bring more than 16 rows a head on average.
+  // Units hold the rows that requests bring a head on average, in eights (at most 32, 16 where D = 256, which
+  // is what the output takes of the registers).
   const int64_t rows = static_cast<int64_t>(a.tokens) * (a.Hq / a.Hkv);
-  const bool two = rows > 16 * static_cast<int64_t>(a.requests);
-  if (a.D == 256) return launch_paged<PagedCfg<T, E4M3, 256, 1>>(a, sms, stream);
-  if (a.D == 128) {
-    return two ? launch_paged<PagedCfg<T, E4M3, 128, 2>>(a, sms, stream) : launch_paged<PagedCfg<T, E4M3, 128, 1>>(a, sms, stream);
+  const int rt = rows <= 8 * static_cast<int64_t>(a.requests) ? 1 : rows <= 16 * static_cast<int64_t>(a.requests) ? 2 : 4;
+  if (a.D == 256) {
+    return rt == 1 ? launch_paged<PagedCfg<T, E4M3, 256, 1>>(a, sms, stream) : launch_paged<PagedCfg<T, E4M3, 256, 2>>(a, sms, stream);
   }
-  return two ? launch_paged<PagedCfg<T, E4M3, 64, 2>>(a, sms, stream) : launch_paged<PagedCfg<T, E4M3, 64, 1>>(a, sms, stream);
+  if (a.D == 128) {
+    return rt == 1   ? launch_paged<PagedCfg<T, E4M3, 128, 1>>(a, sms, stream)
+           : rt == 2 ? launch_paged<PagedCfg<T, E4M3, 128, 2>>(a, sms, stream)
+                     : launch_paged<PagedCfg<T, E4M3, 128, 4>>(a, sms, stream);
+  }
+  return rt == 1   ? launch_paged<PagedCfg<T, E4M3, 64, 1>>(a, sms, stream)
+         : rt == 2 ? launch_paged<PagedCfg<T, E4M3, 64, 2>>(a, sms, stream)
+                   : launch_paged<PagedCfg<T, E4M3, 64, 4>>(a, sms, stream);
 }
 
 template <typename T, bool E4M3>
 static int preload_paged() {
   int rc = configure_paged<PagedCfg<T, E4M3, 64, 1>>();
   if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 64, 2>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 64, 4>>();
   if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 128, 1>>();
   if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 128, 2>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 128, 4>>();
   if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 256, 1>>();
+  if (rc == SYN_OK) rc = configure_paged<PagedCfg<T, E4M3, 256, 2>>();
   return rc;
 }
 

@@ -7,8 +7,9 @@
 // What bounds it.  Every key and value is read once and serves the group of query heads that share it:
 // 4 * group * D operations for 2 * D stored numbers, about `group` operations a byte, against 250 at
 // which the matrix units would become the bound.  So the work is a stream from HBM, the matrix products
-// are small ones (16 rows, padded) on mma.sync, whose fragments stay in registers, and the layout is
-// chosen for loads in flight:
+// are small ones on mma.sync, whose fragments stay in registers; they are turned round (keys by rows,
+// dimensions by rows) because rows then come in eights, as groups do, and not in sixteens.  The layout is chosen
+// for loads in flight:
 //   * Every warp streams keys of its own through a ring of its own in shared memory (cp.async of 16
 //     bytes, a page lookup per key), so no barrier stands between loading and computing; the warps of a
 //     block meet only when a unit of rows ends.
@@ -27,6 +28,7 @@ namespace syn {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
+constexpr int PA_MAX_BLOCKS = 2;  // resident blocks an SM, over all variants
 constexpr int PA_DESC = 8;  // int32 words a block leaves for the join
 
 struct PagedAttnParams {
@@ -38,32 +40,33 @@ struct PagedAttnParams {
   int32_t* desc;      // [grid][PA_DESC]
 };
 
-template <typename T, bool E4M3_, int D_, int MT_>
+template <typename T, bool E4M3_, int D_, int RT_>
 struct PagedCfg {
   using type = T;
   static constexpr bool E4M3 = E4M3_;
   static constexpr int D = D_;
-  static constexpr int MT = MT_;                     // 16-row tiles of a unit
-  static constexpr int ROWS = 16 * MT;
+  static constexpr int RT = RT_;                     // 8-row tiles of a unit
+  static constexpr int ROWS = 8 * RT;
   static constexpr int KEYS = E4M3 ? 32 : 16;        // keys of a warp's step
   static constexpr int TILE = KEYS * PA_WARPS;       // keys of a block's step
   static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
   static constexpr int STEPB = 2 * KEYS * ROWB;      // keys, then values
-  static constexpr int STAGES = D == 64 ? 4 : D == 128 && MT == 2 ? 2 : 3;
+  static constexpr int STAGES = D == 64 ? 4 : D == 128 && RT == 4 ? 2 : 3;
   static constexpr int RING = STAGES * STEPB;        // bytes a warp
-  static constexpr bool QREG = MT == 1 && D <= 128;  // query fragments in registers, else in shared memory
+  static constexpr bool QREG = RT * D <= 256;        // query fragments in registers, else in shared memory
   static constexpr int KSTEPS = D / 16;
-  static constexpr int NT = D / 8;                   // 8-wide output tiles
-  static constexpr int DC = MT == 1 ? 32 : 16;       // output columns of a merge pass
+  static constexpr int DT = D / 16;                  // 16-dimension tiles of the output
+  static constexpr int DC = RT == 1 ? 64 : RT == 2 ? 32 : 16;  // output dimensions of a merge pass
   static constexpr int NT_PASS = DC / 8;
   static constexpr int PASSES = D / DC;
   static constexpr int MERGE_LD = DC + 4;
-  static constexpr int SMEM_Q = QREG ? 0 : KSTEPS * MT * 512;
+  static constexpr int SMEM_Q = QREG ? 0 : KSTEPS * RT * 256;
   static constexpr int SMEM_MERGE = PA_WARPS * ROWS * MERGE_LD * 4;
   static constexpr int SMEM_ML = PA_WARPS * ROWS * 2 * 4;
   static constexpr int SMEM = PA_WARPS * RING + SMEM_Q + SMEM_MERGE + SMEM_ML;
-  static constexpr int BLOCKS = (227 * 1024) / (SMEM + 1024) >= 2 ? 2 : 1;  // resident on an SM
+  static constexpr int FIT = (227 * 1024) / (SMEM + 1280);
+  static constexpr int BLOCKS = FIT < PA_MAX_BLOCKS ? FIT : PA_MAX_BLOCKS;  // resident on an SM
 };
 
 // ----------------------------------------------------------------------------- instructions
@@ -119,10 +122,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two e4m3 bytes as two halves (exact).
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t x) {
+// Four e4m3 bytes as two pairs of halves (exact).
+__device__ __forceinline__ void e4m3x4_to_h2x2(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(x));
+}
+// 8 x 8 matrix of 16-bit numbers, a row in four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 template <bool BF16>
@@ -194,48 +203,51 @@ struct PagedCursor {
 };
 
 // ----------------------------------------------------------------------------- fragments
-// Calls f(nt, b0, b1) with the fragments of 16 keys (group `kk` of the step) for every 8-wide output tile.
-// Output tile nt holds, in its column c, dimension 8 nt + c of 16-bit values.  8-bit values are fetched 16
-// (D = 64: 8) dimensions of one key at a time and paired with the next key's, so there column c of tile nt is
-// dimension 16 c + nt % 16 + 128 (nt / 16) (D = 64: 8 c + nt): a permutation that the epilogue undoes.
+// Calls f(dt, a) with the fragments of the transposed values (16 dimensions by the 16 keys of group `kk` of the
+// step) for every 16-dimension tile of the output.  Row c (0 .. 7) of the tile's halves nt = 2 dt, 2 dt + 1 is
+// dimension 8 nt + c of 16-bit values.  8-bit values are fetched 16 (D = 64: 8) dimensions of one key at a
+// time and paired with the next key's, so there it is dimension 16 c + nt % 16 + 128 (nt / 16) (D = 64:
+// 8 c + nt): a permutation that the epilogue undoes.
 template <typename C, typename F>
 __device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
   if constexpr (!C::E4M3) {
-    const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+    const int row = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
-    for (int j = 0; j < C::D / 16; ++j) {
-      uint32_t b[4];
-      ldsm4t(v + row * C::ROWB + (((j * 2 + (lane >> 4)) ^ (row & 7)) << 4), b);
-      f(2 * j, b[0], b[1]);
-      f(2 * j + 1, b[2], b[3]);
+    for (int j = 0; j < C::DT; ++j) {
+      uint32_t a[4];
+      ldsm4t(v + row * C::ROWB + (((j * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), a);
+      f(j, a);
     }
   } else {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t row0 = v + (kk * 16 + 2 * t) * C::ROWB;
-    auto words = [&](int nt, uint32_t x0, uint32_t x1, uint32_t x8, uint32_t x9) {
+    auto words = [&](int dt, uint32_t x0, uint32_t x1, uint32_t x8, uint32_t x9) {
       const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);
       const uint32_t lo89 = __byte_perm(x8, x9, 0x5140), hi89 = __byte_perm(x8, x9, 0x7362);
-      f(nt, e4m3x2_to_h2(lo01), e4m3x2_to_h2(lo89));
-      f(nt + 1, e4m3x2_to_h2(lo01 >> 16), e4m3x2_to_h2(lo89 >> 16));
-      f(nt + 2, e4m3x2_to_h2(hi01), e4m3x2_to_h2(hi89));
-      f(nt + 3, e4m3x2_to_h2(hi01 >> 16), e4m3x2_to_h2(hi89 >> 16));
+      uint32_t a[4];
+      e4m3x4_to_h2x2(lo01, a[0], a[1]);
+      e4m3x4_to_h2x2(lo89, a[2], a[3]);
+      f(dt, a);
+      e4m3x4_to_h2x2(hi01, a[0], a[1]);
+      e4m3x4_to_h2x2(hi89, a[2], a[3]);
+      f(dt + 1, a);
     };
     if constexpr (C::D == 64) {
       const uint32_t at = (((g >> 1) ^ t) << 4) + (g & 1) * 8;
       const uint2 x0 = lds8(row0 + at), x1 = lds8(row0 + C::ROWB + at);
       const uint2 x8 = lds8(row0 + 8 * C::ROWB + at), x9 = lds8(row0 + 9 * C::ROWB + at);
       words(0, x0.x, x1.x, x8.x, x9.x);
-      words(4, x0.y, x1.y, x8.y, x9.y);
+      words(2, x0.y, x1.y, x8.y, x9.y);
     } else {
 #pragma unroll
       for (int half = 0; half < C::D / 128; ++half) {
         const uint32_t at = ((g + half * 8) ^ (t << 1)) << 4;
         const uint4 x0 = lds16(row0 + at), x1 = lds16(row0 + C::ROWB + at);
         const uint4 x8 = lds16(row0 + 8 * C::ROWB + at), x9 = lds16(row0 + 9 * C::ROWB + at);
-        words(half * 16, x0.x, x1.x, x8.x, x9.x);
-        words(half * 16 + 4, x0.y, x1.y, x8.y, x9.y);
-        words(half * 16 + 8, x0.z, x1.z, x8.z, x9.z);
-        words(half * 16 + 12, x0.w, x1.w, x8.w, x9.w);
+        words(half * 8, x0.x, x1.x, x8.x, x9.x);
+        words(half * 8 + 2, x0.y, x1.y, x8.y, x9.y);
+        words(half * 8 + 4, x0.z, x1.z, x8.z, x9.z);
+        words(half * 8 + 6, x0.w, x1.w, x8.w, x9.w);
       }
     }
   }
@@ -260,7 +272,7 @@ __device__ __forceinline__ int merge_dim(int pass, int e) {
   if constexpr (C::D == 64) return 8 * c + nt;
   return (nt / 16) * 128 + 16 * c + nt % 16;
 }
-// Entry of column c of the pass's i-th output tile.
+// Entry of row c of the pass's i-th 8-dimension tile.
 template <typename C>
 __device__ __forceinline__ int merge_entry(int i, int c) {
   return C::E4M3 ? c * C::NT_PASS + i : i * 8 + c;
@@ -271,7 +283,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   using T = typename C::type;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool MBF16 = BF16 && !C::E4M3;  // type of the matrix products: 8-bit values are halves there
-  constexpr int MT = C::MT;
+  constexpr int RT = C::RT;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_sum[PA_WARPS];
   __shared__ long long s_rest;
@@ -406,16 +418,22 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const int rows = min(C::ROWS, r.n * group - row0);
     const int pos0 = r.len - r.n;
     const int tiles = static_cast<int>(min(static_cast<long long>(r.tiles - cur.tile), t1 - t));
-    int lo[2 * MT], hi[2 * MT];  // keys that rows g, g + 8, ... see
-    float mult[2 * MT];
-    const T* qrow[2 * MT];
+    // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
+    // Rows behind the last repeat it.
+    int lo[2 * RT], hi[2 * RT];
+    float mult[2 * RT];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const int row = row0 + min(g + 8 * i, rows - 1);  // rows behind the last repeat it
-      const int tok = row / group, head = kv_head * group + row - tok * group;
-      hi[i] = a.causal ? min(r.len, pos0 + tok + 1) : r.len;
-      lo[i] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
-      mult[i] = a.sm_scale * CUDART_L2E_F;
+    for (int x = 0; x < 2 * RT; ++x) {
+      const int tok = (row0 + min((x >> 1) * 8 + 2 * t4 + (x & 1), rows - 1)) / group;
+      hi[x] = a.causal ? min(r.len, pos0 + tok + 1) : r.len;
+      lo[x] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
+      mult[x] = a.sm_scale * CUDART_L2E_F;
+      if constexpr (C::E4M3) mult[x] *= a.k_scale[kv_head];
+    }
+    const T* qrow[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int row = row0 + min(8 * i + g, rows - 1), tok = row / group, head = kv_head * group + row - tok * group;
       qrow[i] = static_cast<const T*>(a.q) + static_cast<int64_t>(r.s0 + tok) * a.q_strides[0] + head * a.q_strides[1];
     }
     const int tok_a = row0 / group, tok_b = (row0 + rows - 1) / group;
@@ -423,15 +441,10 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const int all_hi = a.causal ? min(r.len, pos0 + tok_a + 1) : r.len;
 
     // ---- query fragments
-    if constexpr (C::E4M3) {
-      const float ks = a.k_scale[kv_head];
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) mult[i] *= ks;
-    }
-    float up[2 * MT];  // bf16 queries over 8-bit keys: a power of two brings each row into the range of halves
+    float up[RT];  // bf16 queries over 8-bit keys: a power of two brings each row into the range of halves
     if constexpr (C::E4M3 && BF16) {
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) {
+      for (int i = 0; i < RT; ++i) {
         uint32_t top = 0;  // largest magnitude as bits
 #pragma unroll
         for (int c = 0; c < C::D / 32; ++c) {
@@ -445,60 +458,63 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
         const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
         up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        mult[i] *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) mult[2 * i + c] *= __shfl_sync(~0u, down, (2 * t4 + c) * 4);
       }
     }
-    auto q_frag = [&](int ks, int mt, uint32_t (&f)[4]) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const T* q = qrow[2 * mt + half];
-        uint32_t x, y;
-        if constexpr (!C::E4M3) {
-          x = __ldg(reinterpret_cast<const uint32_t*>(q) + ks * 8 + t4);
-          y = __ldg(reinterpret_cast<const uint32_t*>(q) + ks * 8 + t4 + 4);
-        } else {  // the order in which the 8-bit keys are fetched
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + (t4 + ks / 4 * 4) * 4 + ks % 4);
-          x = v.x, y = v.y;
-          if constexpr (BF16) {
-            const float s = up[2 * mt + half];
-            const float2 xf = unpack2<true>(x), yf = unpack2<true>(y);
-            x = pack2<false>(xf.x * s, xf.y * s);
-            y = pack2<false>(yf.x * s, yf.y * s);
-          }
+    auto q_frag = [&](int ks, int i, uint32_t (&f)[2]) {
+      if constexpr (!C::E4M3) {
+        f[0] = __ldg(reinterpret_cast<const uint32_t*>(qrow[i]) + ks * 8 + t4);
+        f[1] = __ldg(reinterpret_cast<const uint32_t*>(qrow[i]) + ks * 8 + t4 + 4);
+      } else {  // the order in which the 8-bit keys are fetched
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(qrow[i]) + (t4 + ks / 4 * 4) * 4 + ks % 4);
+        f[0] = v.x, f[1] = v.y;
+        if constexpr (BF16) {
+          const float2 x = unpack2<true>(v.x), y = unpack2<true>(v.y);
+          f[0] = pack2<false>(x.x * up[i], x.y * up[i]);
+          f[1] = pack2<false>(y.x * up[i], y.y * up[i]);
         }
-        f[half] = x;
-        f[2 + half] = y;
       }
     };
-    uint32_t qreg[C::QREG ? C::KSTEPS : 1][4];
+    uint32_t qreg[C::QREG ? C::KSTEPS * RT : 1][2];
     if constexpr (C::QREG) {
 #pragma unroll
-      for (int ks = 0; ks < C::KSTEPS; ++ks) q_frag(ks, 0, qreg[ks]);
+      for (int ks = 0; ks < C::KSTEPS; ++ks)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) q_frag(ks, i, qreg[ks * RT + i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < C::KSTEPS * MT / PA_WARPS; ++i) {
-        const int f = i * PA_WARPS + warp;
-        uint32_t x[4];
-        if constexpr (MT == 1) {
-          q_frag(f, 0, x);
-        } else {
-          if (f % MT == 0) q_frag(f / MT, 0, x);
-          else q_frag(f / MT, MT - 1, x);
+      for (int j = 0; j < C::KSTEPS / PA_WARPS; ++j) {
+        const int ks = j * PA_WARPS + warp;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          uint32_t f[2];
+          q_frag(ks, i, f);
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(q_smem + (ks * RT + i) * 256 + lane * 8), "r"(f[0]), "r"(f[1])
+                       : "memory");
         }
-        sts16(q_smem + f * 512 + lane * 16, x[0], x[1], x[2], x[3]);
       }
       __syncthreads();
     }
+    auto q_at = [&](int ks, int i, uint32_t (&f)[2]) {
+      if constexpr (C::QREG) {
+        f[0] = qreg[ks * RT + i][0], f[1] = qreg[ks * RT + i][1];
+      } else {
+        const uint2 x = lds8(q_smem + (ks * RT + i) * 256 + lane * 8);
+        f[0] = x.x, f[1] = x.y;
+      }
+    };
 
-    float o[MT][C::NT][4], m[2 * MT], l[2 * MT];
+    float o[C::DT][RT][4], m[2 * RT], l[2 * RT];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) m[i] = -CUDART_INF_F, l[i] = 0.f;
+    for (int x = 0; x < 2 * RT; ++x) m[x] = -CUDART_INF_F, l[x] = 0.f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-      for (int nt = 0; nt < C::NT; ++nt)
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[mt][nt][c] = 0.f;
+        for (int c = 0; c < 4; ++c) o[dt][i][c] = 0.f;
 
     for (int i = 0; i < tiles; ++i) {
       cp_async_wait<C::STAGES - 2>();
@@ -509,53 +525,48 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       const int base = r.first + (cur.tile + i) * C::TILE + warp * C::KEYS;
       if (base >= r.len) continue;
 
-      // ---- scores
-      constexpr int SN = C::KEYS / 8;
-      float s[MT][SN][4];
+      // ---- scores, transposed: 16 keys by 8 rows a product
+      constexpr int SN = C::KEYS / 16;
+      float s[SN][RT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < SN; ++n)
 #pragma unroll
-        for (int n = 0; n < SN; ++n)
+        for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[mt][n][c] = 0.f;
-      auto q_at = [&](int ks, int mt, uint32_t (&f)[4]) {
-        if constexpr (C::QREG) {
-          f[0] = qreg[ks][0], f[1] = qreg[ks][1], f[2] = qreg[ks][2], f[3] = qreg[ks][3];
-        } else {
-          const uint4 x = lds16(q_smem + (ks * MT + mt) * 512 + lane * 16);
-          f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
-        }
-      };
+          for (int c = 0; c < 4; ++c) s[n][j][c] = 0.f;
       if constexpr (!C::E4M3) {
-        const int row = (lane & 7) + (lane >> 4) * 8;
+        const int row = lane & 15;
 #pragma unroll
         for (int ks = 0; ks < C::KSTEPS; ++ks) {
-          uint32_t b[4], f[4];
-          ldsm4(k_at + row * C::ROWB + (((ks * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), b);
+          uint32_t k[4];
+          ldsm4(k_at + row * C::ROWB + (((ks * 2 + (lane >> 4)) ^ (row & 7)) << 4), k);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            q_at(ks, mt, f);
-            mma16816<MBF16>(s[mt][0], f, b[0], b[1]);
-            mma16816<MBF16>(s[mt][1], f, b[2], b[3]);
+          for (int j = 0; j < RT; ++j) {
+            uint32_t f[2];
+            q_at(ks, j, f);
+            mma16816<MBF16>(s[0][j], k, f[0], f[1]);
           }
         }
       } else {
 #pragma unroll
         for (int part = 0; part < C::D / 64; ++part) {
-          uint32_t f[4][MT][4];
+          uint32_t f[4][RT][2];
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) q_at(part * 4 + w, mt, f[w][mt]);
+            for (int j = 0; j < RT; ++j) q_at(part * 4 + w, j, f[w][j]);
 #pragma unroll
           for (int n = 0; n < SN; ++n) {
-            const uint4 x = lds16(k_at + ring_at<C, false>(n * 8 + g, t4 + part * 4));
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            const uint4 x = lds16(k_at + ring_at<C, false>(n * 16 + g, t4 + part * 4));
+            const uint4 y = lds16(k_at + ring_at<C, false>(n * 16 + 8 + g, t4 + part * 4));
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t b0 = e4m3x2_to_h2(w[j]), b1 = e4m3x2_to_h2(w[j] >> 16);
+            for (int w = 0; w < 4; ++w) {
+              uint32_t k[4];
+              e4m3x4_to_h2x2(xw[w], k[0], k[2]);
+              e4m3x4_to_h2x2(yw[w], k[1], k[3]);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) mma16816<false>(s[mt][n], f[j][mt], b0, b1);
+              for (int j = 0; j < RT; ++j) mma16816<false>(s[n][j], k, f[w][j][0], f[w][j][1]);
             }
           }
         }
@@ -563,101 +574,108 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
       // ---- weights
       const bool whole = base >= all_lo && base + C::KEYS <= all_hi;  // every row sees every key
-      float alpha[2 * MT];
+      float alpha[2 * RT];
       bool rose = false;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int x = 0; x < 2 * RT; ++x) {
+        float top = m[x];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int x = 2 * mt + half;
-          float top = m[x];
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int n = 0; n < SN; ++n)
+          for (int h = 0; h < 2; ++h) {
+            float& v = s[n][x >> 1][2 * h + (x & 1)];
+            v *= mult[x];
+            const int key = base + n * 16 + h * 8 + g;
+            if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
+            top = fmaxf(top, v);
+          }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+        rose |= top > m[x];
+        const float zero = top == -CUDART_INF_F ? 0.f : top;
+        alpha[x] = ex2(m[x] - zero);
+        m[x] = top;
+        float sum = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float& v = s[mt][n][2 * half + c];
-              v *= mult[x];
-              const int key = base + n * 8 + t4 * 2 + c;
-              if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
-              top = fmaxf(top, v);
-            }
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-          rose |= top > m[x];
-          const float zero = top == -CUDART_INF_F ? 0.f : top;
-          alpha[x] = ex2(m[x] - zero);
-          m[x] = top;
-          float sum = 0.f;
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int n = 0; n < SN; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float& v = s[mt][n][2 * half + c];
-              v = ex2(v - zero);
-              sum += v;
-            }
-          l[x] = l[x] * alpha[x] + sum;
-        }
+          for (int h = 0; h < 2; ++h) {
+            float& v = s[n][x >> 1][2 * h + (x & 1)];
+            v = ex2(v - zero);
+            sum += v;
+          }
+        l[x] = l[x] * alpha[x] + sum;
+      }
       if (__any_sync(~0u, rose)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-          for (int nt = 0; nt < C::NT; ++nt)
+          for (int j = 0; j < RT; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[mt][nt][c] *= alpha[2 * mt + c / 2];
+            for (int c = 0; c < 4; ++c) o[dt][j][c] *= alpha[2 * j + (c & 1)];
       }
 
-      // ---- values.  The weights enter the product as two 16-bit numbers, the second one what the first
-      // left, so that their rounding (2^-9 alone) does not add to that of the output.
+      // ---- values, transposed: 16 dimensions by 8 rows a product.  The weights enter as two 16-bit numbers, the
+      // second one what the first left, so that their rounding does not add to that of the output.
+#ifndef PA_LOW
+#define PA_LOW true
+#endif
+      constexpr bool LOW = PA_LOW;
 #pragma unroll
-      for (int kk = 0; kk < C::KEYS / 16; ++kk) {
-        uint32_t ph[MT][4], pl[MT][4];
+      for (int kk = 0; kk < SN; ++kk) {
+        uint32_t ph[RT][2], pl[RT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float* v = &s[mt][2 * kk + (q >> 1)][2 * (q & 1)];
-            ph[mt][q] = pack2<MBF16>(v[0], v[1]);
-            const float2 b = unpack2<MBF16>(ph[mt][q]);
-            pl[mt][q] = pack2<MBF16>(v[0] - b.x, v[1] - b.y);
+          for (int h = 0; h < 2; ++h) {
+            const float x = s[kk][j][2 * h], y = s[kk][j][2 * h + 1];
+            const uint32_t top = pack2<MBF16>(x, y);
+            ph[j][h] = transpose8(top);
+            if constexpr (LOW) {
+              const float2 b = unpack2<MBF16>(top);
+              pl[j][h] = transpose8(pack2<MBF16>(x - b.x, y - b.y));
+            }
           }
         bool odd = false;  // values that are not finite, at keys that not every row sees
         if (!whole && r.n > 1) {
           constexpr uint32_t EXP = MBF16 ? 0x7F807F80u : 0x7C007C00u, ONE = MBF16 ? 0x00800080u : 0x04000400u;
-          each_v<C>(v_at, lane, kk, [&](int, uint32_t b0, uint32_t b1) {
-            odd |= ((((b0 & EXP) + ONE) | ((b1 & EXP) + ONE)) & 0x80008000u) != 0;
+          each_v<C>(v_at, lane, kk, [&](int, const uint32_t (&v)[4]) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) odd |= (((v[c] & EXP) + ONE) & 0x80008000u) != 0;
           });
           odd = __any_sync(~0u, odd);
         }
         if (!odd) {
-          each_v<C>(v_at, lane, kk, [&](int nt, uint32_t b0, uint32_t b1) {
+          each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<MBF16>(o[mt][nt], ph[mt], b0, b1);
-              mma16816<MBF16>(o[mt][nt], pl[mt], b0, b1);
+            for (int j = 0; j < RT; ++j) {
+              mma16816<MBF16>(o[dt][j], v, ph[j][0], ph[j][1]);
+              if constexpr (LOW) mma16816<MBF16>(o[dt][j], v, pl[j][0], pl[j][1]);
             }
           });
         } else {
           // Zero times infinity: such values may only enter the rows that see them, so one row at a time,
           // with what it does not see taken out.
 #pragma unroll
-          for (int x = 0; x < 2 * MT; ++x) {
-            const int mt = x >> 1, half = x & 1;
+          for (int x = 0; x < 2 * RT; ++x) {
+            const int j = x >> 1;
 #pragma unroll 1
-            for (int row = 0; row < 8; ++row) {
-              const int row_lo = __shfl_sync(~0u, lo[x], row * 4), row_hi = __shfl_sync(~0u, hi[x], row * 4);
+            for (int q = 0; q < 4; ++q) {  // row 8 j + 2 q + (x & 1), a column of lanes t4 == q
+              const int row_lo = __shfl_sync(~0u, lo[x], q), row_hi = __shfl_sync(~0u, hi[x], q);
               const int key = base + kk * 16 + t4 * 2;
               auto seen = [&](int k) {
                 return (k >= row_lo && k < row_hi ? 0xFFFFu : 0u) | (k + 1 >= row_lo && k + 1 < row_hi ? 0xFFFF0000u : 0u);
               };
               const uint32_t mask0 = seen(key), mask1 = seen(key + 8);
-              each_v<C>(v_at, lane, kk, [&](int nt, uint32_t b0, uint32_t b1) {
+              each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
+                const uint32_t u[4] = {v[0] & mask0, v[1] & mask0, v[2] & mask1, v[3] & mask1};
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<MBF16>(c, ph[mt], b0 & mask0, b1 & mask1);
-                mma16816<MBF16>(c, pl[mt], b0 & mask0, b1 & mask1);
-                if (g == row) {
-                  o[mt][nt][2 * half] += c[2 * half];
-                  o[mt][nt][2 * half + 1] += c[2 * half + 1];
+                mma16816<MBF16>(c, u, ph[j][0], ph[j][1]);
+                if constexpr (LOW) mma16816<MBF16>(c, u, pl[j][0], pl[j][1]);
+                if (t4 == q) {
+                  o[dt][j][x & 1] += c[x & 1];
+                  o[dt][j][2 + (x & 1)] += c[2 + (x & 1)];
                 }
               });
             }
@@ -668,22 +686,25 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
     // ---- the warps' parts of the unit are put together
 #pragma unroll
-    for (int x = 0; x < 2 * MT; ++x) {
-      l[x] += __shfl_xor_sync(~0u, l[x], 1);
-      l[x] += __shfl_xor_sync(~0u, l[x], 2);
-      if (t4 == 0) s_m[warp * C::ROWS + g + 8 * x] = m[x], s_l[warp * C::ROWS + g + 8 * x] = l[x];
+    for (int x = 0; x < 2 * RT; ++x) {
+      l[x] += __shfl_xor_sync(~0u, l[x], 4);
+      l[x] += __shfl_xor_sync(~0u, l[x], 8);
+      l[x] += __shfl_xor_sync(~0u, l[x], 16);
+      const int row = (x >> 1) * 8 + 2 * t4 + (x & 1);
+      if (g == 0) s_m[warp * C::ROWS + row] = m[x], s_l[warp * C::ROWS + row] = l[x];
     }
     __syncthreads();
 #pragma unroll
-    for (int x = 0; x < 2 * MT; ++x) {
+    for (int x = 0; x < 2 * RT; ++x) {
+      const int row = (x >> 1) * 8 + 2 * t4 + (x & 1);
       float top = -CUDART_INF_F;
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + g + 8 * x]);
+      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + row]);
       const float f = ex2(m[x] - (top == -CUDART_INF_F ? 0.f : top));
 #pragma unroll
-      for (int nt = 0; nt < C::NT; ++nt) {
-        o[x >> 1][nt][2 * (x & 1)] *= f;
-        o[x >> 1][nt][2 * (x & 1) + 1] *= f;
+      for (int dt = 0; dt < C::DT; ++dt) {
+        o[dt][x >> 1][x & 1] *= f;
+        o[dt][x >> 1][2 + (x & 1)] *= f;
       }
     }
     constexpr int TPR = C::DC / 4;  // threads a row
@@ -715,14 +736,15 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     for (int pass = 0; pass < C::PASSES; ++pass) {
       if (pass > 0) __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 2 * MT; ++x) {
-        if (g + 8 * x < rows) {
-          float* to = merge + (warp * C::ROWS + g + 8 * x) * C::MERGE_LD;
+      for (int x = 0; x < 2 * RT; ++x) {
+        const int to_row = (x >> 1) * 8 + 2 * t4 + (x & 1);
+        if (to_row < rows) {
+          float* to = merge + (warp * C::ROWS + to_row) * C::MERGE_LD;
 #pragma unroll
-          for (int n = 0; n < C::NT_PASS; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              to[merge_entry<C>(n, t4 * 2 + c)] = o[x >> 1][pass * C::NT_PASS + n][2 * (x & 1) + c];
+          for (int n = 0; n < C::NT_PASS; ++n) {
+            const int nt = pass * C::NT_PASS + n;
+            to[merge_entry<C>(n, g)] = o[nt >> 1][x >> 1][2 * (nt & 1) + (x & 1)];
+          }
         }
       }
       __syncthreads();
@@ -776,12 +798,17 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 }
 
 // Joins the parts of the units that borders between blocks cut: block c takes the unit that the border
-// before block c + 1 cuts, if that is the first border in it.  A warp takes a row.
+// before block c + 1 cuts, if that is the first border in it.  With few rows several warps share a row and
+// take its parts in turn (a long request has dozens), so that few loads wait for one another.
+constexpr int PA_JOIN_WARPS = 16;
+
 template <typename C>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
   using T = typename C::type;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int N = C::D / 64;  // pairs of columns a lane
+  __shared__ float2 s_o[PA_JOIN_WARPS][C::D / 2];
+  __shared__ float s_m[PA_JOIN_WARPS], s_l[PA_JOIN_WARPS];
   const syn_paged_attn_args& a = p.a;
   const int c = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -792,36 +819,78 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   const PagedRequest r = paged_request<C>(a, z);
   const int group = a.Hq / a.Hkv, kv_head = sub / r.rt, row0 = (sub - kv_head * r.rt) * C::ROWS;
   const int rows = min(C::ROWS, r.n * group - row0);
+  int wide = 1;  // warps a row
+  while (wide * 2 * rows <= PA_JOIN_WARPS && wide * 2 <= parts) wide *= 2;
+  const int share = warp % wide;
   auto slot = [&](int i) { return i == 0 ? before.y : 2 * (c - 1 + i); };
-  for (int row = warp; row < rows; row += 8) {
-    float top = -CUDART_INF_F;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[(slot(i) * C::ROWS + row) * 2]);
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    const float zero = top == -CUDART_INF_F ? 0.f : top;
-    float sum = 0.f;
+  for (int first = 0; first < rows; first += PA_JOIN_WARPS / wide) {
+    const int row = first + warp / wide;
+    const bool live = row < rows;
+    float top = -CUDART_INF_F, sum = 0.f;
     float2 v[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const int64_t at = static_cast<int64_t>(slot(i)) * C::ROWS + row;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float w = ex2(ml.x - zero);
-      sum += ml.y * w;
+    if (live) {
+      for (int i0 = share; i0 < parts; i0 += 32 * wide) {  // a part's statistics a lane, then one part after the other
+        const int i = i0 + lane * wide;
+        float2 ml = make_float2(-CUDART_INF_F, 0.f);
+        if (i < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + (static_cast<int64_t>(slot(i)) * C::ROWS + row) * 2);
+        float now = fmaxf(top, ml.x);
+        for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(~0u, now, d));
+        const float zero = now == -CUDART_INF_F ? 0.f : now, alpha = ex2(top - zero);
+        top = now;
+        const float w = ex2(ml.x - zero);
+        float more = ml.y * w;
+        for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(~0u, more, d);
+        sum = sum * alpha + more;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float2 u = *reinterpret_cast<const float2*>(p.part_o + at * C::D + j * 64 + lane * 2);
-        v[j].x += u.x * w, v[j].y += u.y * w;
+        for (int j = 0; j < N; ++j) v[j].x *= alpha, v[j].y *= alpha;
+        const int count = min(32, (parts - i0 + wide - 1) / wide);
+#pragma unroll 8
+        for (int k = 0; k < count; ++k) {
+          const float f = __shfl_sync(~0u, w, k);
+          const float* from = p.part_o + (static_cast<int64_t>(slot(i0 + k * wide)) * C::ROWS + row) * C::D + lane * 2;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float2 u = *reinterpret_cast<const float2*>(from + j * 64);
+            v[j].x += u.x * f, v[j].y += u.y * f;
+          }
+        }
       }
     }
-    float factor = sum == 0.f ? 0.f : 1.f / sum;
-    if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
-    const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
-    T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+    if (wide > 1) {
+      __syncthreads();
+      if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
-    if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+      for (int j = 0; j < N; ++j) s_o[warp][j * 32 + lane] = v[j];
+      __syncthreads();
+      if (live && share == 0) {
+        for (int w = 1; w < wide; ++w) top = fmaxf(top, s_m[warp + w]);
+        const float zero = top == -CUDART_INF_F ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
+        for (int w = 0; w < wide; ++w) {
+          const float f = ex2(s_m[warp + w] - zero);
+          sum += s_l[warp + w] * f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float2 u = s_o[warp + w][j * 32 + lane];
+            v[j].x += u.x * f, v[j].y += u.y * f;
+          }
+        }
+      }
+    }
+    if (live && share == 0) {
+      float factor = sum == 0.f ? 0.f : 1.f / sum;
+      if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
+      const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
+      T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
+      if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+    }
   }
 }
 
