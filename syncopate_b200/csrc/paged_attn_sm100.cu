@@ -5,12 +5,12 @@
 
 namespace syn {
 
-constexpr int PA_MAX_UNIT = 32 * 128;     // rows x D of a unit, over all variants
-constexpr int PA_MAX_ROWS = 32;
+// Most rows, and rows x D, of the units of an SM's resident blocks, over all variants.
+constexpr int PA_MAX_ROWS = 64;
+constexpr int PA_MAX_SIZE = 64 * 128;
 
 static int64_t paged_workspace(int sms) {
-  const int64_t grid = static_cast<int64_t>(sms) * PA_MAX_BLOCKS;
-  return grid * PA_DESC * 4 + 2 * grid * (PA_MAX_ROWS * 2 + PA_MAX_UNIT) * 4;
+  return static_cast<int64_t>(sms) * (PA_MAX_BLOCKS * PA_DESC + 2 * (PA_MAX_ROWS * 2 + PA_MAX_SIZE)) * 4;
 }
 
 // Opts the kernel into its shared memory, once a device.
@@ -30,12 +30,22 @@ static int configure_paged() {
 
 template <typename C>
 static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stream) {
+  static_assert(C::BLOCKS <= PA_MAX_BLOCKS && C::BLOCKS * C::ROWS <= PA_MAX_ROWS && C::BLOCKS * C::ROWS * C::D <= PA_MAX_SIZE,
+                "workspace");
   int rc = configure_paged<C>();
   if (rc != SYN_OK) return rc;
   PagedAttnParams p;
   p.a = a;
-  p.grid = sms * C::BLOCKS;
+  p.grid = sms * C::BLOCKS < PA_JOIN_MAX ? sms * C::BLOCKS : PA_JOIN_MAX;
   p.min_tiles = 4;
+  // mulhi(n, 2^(31 + b) / d rounded up) >> (b - 1) = n / d for 0 <= n < 2^31, 2^(b - 1) < d <= 2^b
+  p.page_mul = 0, p.page_shift = 0;
+  if (a.page_size > 1) {
+    int b = 1;
+    while ((1ll << b) < a.page_size) ++b;
+    p.page_mul = static_cast<uint32_t>(((1ull << (31 + b)) + a.page_size - 1) / a.page_size);
+    p.page_shift = b - 1;
+  }
   p.desc = static_cast<int32_t*>(a.workspace);
   p.part_ml = reinterpret_cast<float*>(p.desc + p.grid * PA_DESC);
   p.part_o = p.part_ml + static_cast<int64_t>(2) * p.grid * C::ROWS * 2;
@@ -47,7 +57,7 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(p.grid - 1);
+  config.gridDim = dim3(sms);
   config.blockDim = dim3(PA_JOIN_WARPS * 32);
   config.stream = stream;
   config.attrs = &attr;

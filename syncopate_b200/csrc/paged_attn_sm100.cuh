@@ -1,8 +1,8 @@
 // Attention of the newest tokens over a paged key-value cache (decoding, drafted tokens).
 //
-// Mathematics.  Rows are (new token, query head) pairs.  Over its keys in any order a row keeps the
-// running maximum m of its scores (times log2 e), the sum l of 2^(s - m) and the output o = sum 2^(s - m) v,
-// rescaled by 2^(m - m') when the maximum rises; parts of a row's keys are joined by the same rule.
+// Mathematics.  Rows are (new token, query head) pairs.  Over its keys in any order a row keeps a reference m
+// near the maximum of its scores s (times log2 e), the sum l of 2^(s - m) and the output o = sum 2^(s - m) v, rescaled
+// by 2^(m - m') when the reference rises; parts of a row's keys are joined by the same rule.
 //
 // What bounds it.  Every key and value is read once and serves the group of query heads that share it:
 // 4 * group * D operations for 2 * D stored numbers, about `group` operations a byte, against 250 at
@@ -28,13 +28,18 @@ namespace syn {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
-constexpr int PA_MAX_BLOCKS = 2;  // resident blocks an SM, over all variants
-constexpr int PA_DESC = 8;  // int32 words a block leaves for the join
+constexpr int PA_MAX_BLOCKS = 3;  // resident blocks an SM, over all variants
+// The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
+// than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
+constexpr float PA_SLACK = 8.f;
+constexpr int PA_DESC = 4;  // int32 words a block leaves for the join
 
 struct PagedAttnParams {
   syn_paged_attn_args a;
   int32_t grid;       // blocks of the launch
   int32_t min_tiles;  // fewest key tiles worth a block
+  uint32_t page_mul;  // key / page_size = mulhi(key, page_mul) >> page_shift (page_mul 0: pages of one key)
+  int32_t page_shift;
   float* part_o;      // [2 * grid][rows of a unit][D]
   float* part_ml;     // [2 * grid][rows of a unit][2]
   int32_t* desc;      // [grid][PA_DESC]
@@ -51,13 +56,14 @@ struct PagedCfg {
   static constexpr int TILE = KEYS * PA_WARPS;       // keys of a block's step
   static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
-  static constexpr int STEPB = 2 * KEYS * ROWB;      // keys, then values
-  static constexpr int STAGES = D == 64 ? 4 : D == 128 && RT == 4 ? 2 : 3;
-  static constexpr int RING = STAGES * STEPB;        // bytes a warp
+  static constexpr int HALFB = KEYS * ROWB;          // the keys of a step, or its values
+  static constexpr int BLOCKS = D == 256 ? 3 - RT : RT <= 2 ? 3 : 2;  // resident on an SM
+  static constexpr int SLOTS = (D == 256 ? 24 : RT <= 2 ? 16 : 20) * 1024 / HALFB;
+  static constexpr int RING = SLOTS * HALFB;         // bytes a warp
   static constexpr bool QREG = RT * D <= 256;        // query fragments in registers, else in shared memory
   static constexpr int KSTEPS = D / 16;
   static constexpr int DT = D / 16;                  // 16-dimension tiles of the output
-  static constexpr int DC = RT == 1 ? 64 : RT == 2 ? 32 : 16;  // output dimensions of a merge pass
+  static constexpr int DC = RT == 4 ? 16 : 32;  // output dimensions of a merge pass
   static constexpr int NT_PASS = DC / 8;
   static constexpr int PASSES = D / DC;
   static constexpr int MERGE_LD = DC + 4;
@@ -65,13 +71,13 @@ struct PagedCfg {
   static constexpr int SMEM_MERGE = PA_WARPS * ROWS * MERGE_LD * 4;
   static constexpr int SMEM_ML = PA_WARPS * ROWS * 2 * 4;
   static constexpr int SMEM = PA_WARPS * RING + SMEM_Q + SMEM_MERGE + SMEM_ML;
-  static constexpr int FIT = (227 * 1024) / (SMEM + 1280);
-  static constexpr int BLOCKS = FIT < PA_MAX_BLOCKS ? FIT : PA_MAX_BLOCKS;  // resident on an SM
+  static_assert(BLOCKS * (SMEM + 1280) <= 228 * 1024, "shared memory of an SM");
+  static_assert(SLOTS >= 3, "a key half, a value half and one on its way");
 };
 
 // ----------------------------------------------------------------------------- instructions
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   const long long t0 = block < shares ? paged_border(total, shares, block) : total;
   const long long t1 = block < shares ? paged_border(total, shares, block + 1) : total;
   if (t0 >= t1) {
-    if (tid < PA_DESC) p.desc[block * PA_DESC + tid] = 0;
+    if (tid == 0) *reinterpret_cast<int4*>(p.desc + block * PA_DESC) = make_int4(0, 0, 0, -1);
     return;
   }
   if (upto - mine <= t0 && t0 < upto) {
@@ -343,71 +349,96 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   PagedCursor<C> cur;
   cur.at(a, s_z, s_rest);
 
-  // ---- producer: loads run STAGES - 1 steps ahead, across units
+  // ---- producer: halves of steps (keys, values, keys, ...) are asked for SLOTS - 1 halves ahead, across units
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   PagedCursor<C> ahead = cur;
   long long t_ahead = t0;
-  int page = -2, inside = 0;  // page of this lane's key (-2: none), slot in it
-  int head_ahead = ahead.sub / max(ahead.r.rt, 1);
+  int page = -2, inside = 0;  // page of key (lane % KEYS) of the next step (-2: no such key), slot in it
+  int head_ahead = ahead.sub / ahead.r.rt;
+  constexpr int EB = C::E4M3 ? 1 : 2, RPI = 32 / C::CPR == 0 ? 1 : 32 / C::CPR, LOADS = C::HALFB / 512;
   auto look_up = [&]() {
     page = -2;
     if (t_ahead < t1) {
       const int key = ahead.r.first + ahead.tile * C::TILE + warp * C::KEYS + (lane & (C::KEYS - 1));
       if (key < ahead.r.len) {
-        const int i = key / a.page_size;
+        const int i = p.page_mul ? __umulhi(key, p.page_mul) >> p.page_shift : key;
         inside = key - i * a.page_size;
         page = i < a.width ? __ldg(a.table + ahead.z * a.table_stride + i) : -1;
       }
     }
   };
-  auto issue = [&](int stage) {
+  long long off = -2;     // byte offset of this lane's key in the caches (-2: no such key, -1: no such page)
+  bool one_page = false;  // the step's keys lie behind one another in one page, all of them there
+  auto issue = [&](uint32_t slot, bool values) {
     if (t_ahead < t1) {
-      long long off = -2;
-      if (page != -2) {
-        if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) {
-          off = page * a.cache_strides[0] + inside * a.cache_strides[1] + head_ahead * a.cache_strides[2];
-          if (C::E4M3 == false) off *= 2;
-        } else {
-          off = -1;
-          paged_record(a.status, SYN_DEV_BAD_INDEX, ahead.z, page);
+      if (!values) {
+        off = -2;
+        if (page != -2) {
+          if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) {
+            off = (page * a.cache_strides[0] + inside * a.cache_strides[1] + head_ahead * a.cache_strides[2]) * EB;
+          } else {
+            off = -1;
+            paged_record(a.status, SYN_DEV_BAD_INDEX, ahead.z, page);
+          }
         }
+        const int last = __shfl_sync(~0u, inside, C::KEYS - 1), from = __shfl_sync(~0u, inside, 0);
+        one_page = __all_sync(~0u, off >= 0) && last == from + C::KEYS - 1;
+        if (one_page)  // a lane's own place: row lane / CPR, chunk lane % CPR
+          off = __shfl_sync(~0u, off, 0) + (lane / C::CPR) * a.cache_strides[1] * EB + lane % C::CPR * 16;
       }
-      const uint32_t slot = ring + stage * C::STEPB;
+      const char* base = static_cast<const char*>(values ? a.v_cache : a.k_cache);
+      if (one_page) {
+        const char* from = base + off;
+        const int64_t skip = RPI * a.cache_strides[1] * EB;
 #pragma unroll
-      for (int i = 0; i < C::KEYS * C::CPR / 32; ++i) {
-        const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
-        const long long o = __shfl_sync(~0u, off, row);
-        const uint32_t kd = slot + ring_at<C, false>(row, chunk), vd = slot + C::KEYS * C::ROWB + ring_at<C, true>(row, chunk);
-        if (o != -1) {
-          const long long at = o < 0 ? 0 : o + chunk * 16;
-          const uint32_t bytes = o < 0 ? 0 : 16;  // keys behind the end come as zeros
-          cp_async16(kd, static_cast<const char*>(a.k_cache) + at, bytes);
-          cp_async16(vd, static_cast<const char*>(a.v_cache) + at, bytes);
-        } else {  // no such page: NaN in every type
-          sts16(kd, ~0u, ~0u, ~0u, ~0u);
-          sts16(vd, ~0u, ~0u, ~0u, ~0u);
+        for (int i = 0; i < LOADS; ++i) {
+          const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
+          cp_async16(slot + (values ? ring_at<C, true>(row, chunk) : ring_at<C, false>(row, chunk)), from);
+          from += skip;
+        }
+      } else {
+#pragma unroll 2
+        for (int i = 0; i < LOADS; ++i) {
+          const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
+          const long long o = __shfl_sync(~0u, off, row);
+          const uint32_t to = slot + (values ? ring_at<C, true>(row, chunk) : ring_at<C, false>(row, chunk));
+          if (o == -1) sts16(to, ~0u, ~0u, ~0u, ~0u);  // no such page: NaN in every type
+          else if (o == -2) sts16(to, 0, 0, 0, 0);     // keys behind the end come as zeros
+          else cp_async16(to, base + o + chunk * 16);
         }
       }
-      ++t_ahead;
-      if (++ahead.tile == ahead.r.tiles) {
-        if (t_ahead < t1) ahead.next_unit(a);
-        head_ahead = ahead.sub / ahead.r.rt;
+      if (values) {
+        ++t_ahead;
+        if (++ahead.tile == ahead.r.tiles) {
+          if (t_ahead < t1) ahead.next_unit(a);
+          head_ahead = ahead.sub / ahead.r.rt;
+        }
+        look_up();
       }
-      look_up();
     }
     cp_async_commit();
   };
   look_up();
 #pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+  for (int s = 0; s < C::SLOTS - 1; ++s) issue(ring + s * C::HALFB, s & 1);
+  // Slot of the half being read; the one read before it is the next to fill.
+  int slot = 0;
+  auto next_half = [&](bool values) {
+    cp_async_wait<C::SLOTS - 2>();
+    __syncwarp();
+    const uint32_t at = ring + slot * C::HALFB;
+    issue(ring + (slot == 0 ? C::SLOTS - 1 : slot - 1) * C::HALFB, (C::SLOTS & 1) ? values : !values);
+    if (++slot == C::SLOTS) slot = 0;
+    return at;
+  };
 
   const uint32_t q_smem = smem_u32(smem) + PA_WARPS * C::RING;
   float* merge = reinterpret_cast<float*>(smem + PA_WARPS * C::RING + C::SMEM_Q);
   float* s_m = merge + C::SMEM_MERGE / 4;  // [warp][row]
   float* s_l = s_m + PA_WARPS * C::ROWS;
-  int stage = 0;
   long long t = t0;
-  int first_open = 0, first_mid = 0, parts = 0, tail_from_start = 0, tail_slot = 0;
+  int parts = 0;       // of the unit that this block comes in in the middle of, from the block before on
+  int tail_slot = -1;  // part of the unit that it begins and does not end
   const int z_first = cur.z, sub_first = cur.sub;
   bool first_segment = true;
 
@@ -517,13 +548,12 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int c = 0; c < 4; ++c) o[dt][i][c] = 0.f;
 
     for (int i = 0; i < tiles; ++i) {
-      cp_async_wait<C::STAGES - 2>();
-      __syncwarp();
-      issue(stage == 0 ? C::STAGES - 1 : stage - 1);  // into the slot read in the step before
-      const uint32_t k_at = ring + stage * C::STEPB, v_at = k_at + C::KEYS * C::ROWB;
-      if (++stage == C::STAGES) stage = 0;
+      const uint32_t k_at = next_half(false);
       const int base = r.first + (cur.tile + i) * C::TILE + warp * C::KEYS;
-      if (base >= r.len) continue;
+      if (base >= r.len) {  // no key of this warp
+        next_half(true);
+        continue;
+      }
 
       // ---- scores, transposed: 16 keys by 8 rows a product
       constexpr int SN = C::KEYS / 16;
@@ -574,11 +604,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
       // ---- weights
       const bool whole = base >= all_lo && base + C::KEYS <= all_hi;  // every row sees every key
-      float alpha[2 * RT];
-      bool rose = false;
+      bool rise = false;
 #pragma unroll
-      for (int x = 0; x < 2 * RT; ++x) {
-        float top = m[x];
+      for (int x = 0; x < 2 * RT; ++x)
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
@@ -587,41 +615,43 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
             v *= mult[x];
             const int key = base + n * 16 + h * 8 + g;
             if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
-            top = fmaxf(top, v);
+            rise |= v > m[x] + PA_SLACK;
           }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-        rose |= top > m[x];
-        const float zero = top == -CUDART_INF_F ? 0.f : top;
-        alpha[x] = ex2(m[x] - zero);
-        m[x] = top;
-        float sum = 0.f;
+      if (__any_sync(~0u, rise)) {
+#pragma unroll
+        for (int x = 0; x < 2 * RT; ++x) {
+          float top = m[x];
+#pragma unroll
+          for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[n][x >> 1][x & 1], s[n][x >> 1][2 + (x & 1)]));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          const float alpha = ex2(m[x] - (top == -CUDART_INF_F ? 0.f : top));
+          m[x] = top;
+          l[x] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < C::DT; ++dt) {
+            o[dt][x >> 1][x & 1] *= alpha;
+            o[dt][x >> 1][2 + (x & 1)] *= alpha;
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2 * RT; ++x) {
+        const float zero = m[x] == -CUDART_INF_F ? 0.f : m[x];
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float& v = s[n][x >> 1][2 * h + (x & 1)];
             v = ex2(v - zero);
-            sum += v;
+            l[x] += v;
           }
-        l[x] = l[x] * alpha[x] + sum;
       }
-      if (__any_sync(~0u, rose)) {
-#pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-          for (int j = 0; j < RT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[dt][j][c] *= alpha[2 * j + (c & 1)];
-      }
+      const uint32_t v_at = next_half(true);
 
       // ---- values, transposed: 16 dimensions by 8 rows a product.  The weights enter as two 16-bit numbers, the
       // second one what the first left, so that their rounding does not add to that of the output.
-#ifndef PA_LOW
-#define PA_LOW true
-#endif
-      constexpr bool LOW = PA_LOW;
 #pragma unroll
       for (int kk = 0; kk < SN; ++kk) {
         uint32_t ph[RT][2], pl[RT][2];
@@ -632,10 +662,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
             const float x = s[kk][j][2 * h], y = s[kk][j][2 * h + 1];
             const uint32_t top = pack2<MBF16>(x, y);
             ph[j][h] = transpose8(top);
-            if constexpr (LOW) {
-              const float2 b = unpack2<MBF16>(top);
-              pl[j][h] = transpose8(pack2<MBF16>(x - b.x, y - b.y));
-            }
+            const float2 b = unpack2<MBF16>(top);
+            pl[j][h] = transpose8(pack2<MBF16>(x - b.x, y - b.y));
           }
         bool odd = false;  // values that are not finite, at keys that not every row sees
         if (!whole && r.n > 1) {
@@ -651,7 +679,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
               mma16816<MBF16>(o[dt][j], v, ph[j][0], ph[j][1]);
-              if constexpr (LOW) mma16816<MBF16>(o[dt][j], v, pl[j][0], pl[j][1]);
+              mma16816<MBF16>(o[dt][j], v, pl[j][0], pl[j][1]);
             }
           });
         } else {
@@ -672,7 +700,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
                 const uint32_t u[4] = {v[0] & mask0, v[1] & mask0, v[2] & mask1, v[3] & mask1};
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
                 mma16816<MBF16>(c, u, ph[j][0], ph[j][1]);
-                if constexpr (LOW) mma16816<MBF16>(c, u, pl[j][0], pl[j][1]);
+                mma16816<MBF16>(c, u, pl[j][0], pl[j][1]);
                 if (t4 == q) {
                   o[dt][j][x & 1] += c[x & 1];
                   o[dt][j][2 + (x & 1)] += c[2 + (x & 1)];
@@ -708,7 +736,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       }
     }
     constexpr int TPR = C::DC / 4;  // threads a row
-    const int row = tid / TPR, entry = (tid % TPR) * 4;
+    static_assert(C::ROWS * TPR <= PA_THREADS, "a thread for every four outputs of a pass");
+    const bool writer = tid < C::ROWS * TPR;
+    const int row = writer ? tid / TPR : 0, entry = (tid % TPR) * 4;
     float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + row]);
@@ -722,7 +752,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       factor = sum == 0.f ? 0.f : 1.f / sum;
       if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
     }
-    if (row < rows && entry == 0) {
+    if (writer && row < rows && entry == 0) {
       if (partial) {
         p.part_ml[(part * C::ROWS + row) * 2] = top;
         p.part_ml[(part * C::ROWS + row) * 2 + 1] = sum;
@@ -748,7 +778,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         }
       }
       __syncthreads();
-      if (row < rows) {
+      if (writer && row < rows) {
         float4 v = *reinterpret_cast<const float4*>(merge + row * C::MERGE_LD + entry);
 #pragma unroll
         for (int w = 1; w < PA_WARPS; ++w) {
@@ -768,69 +798,100 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     __syncthreads();
 
     // ---- what the join needs to know
-    if (first_segment) {
-      first_mid = !from_start;
-      first_open = !to_end;
-      if (first_mid) {  // the block that holds the unit's last tile
-        const long long end = t + (r.tiles - cur.tile);
-        int c = static_cast<int>(min((end * shares - 1) / total, static_cast<long long>(shares - 1)));
-        while (c + 1 < shares && paged_border(total, shares, c + 1) < end) ++c;
-        while (paged_border(total, shares, c) >= end) --c;
-        parts = c - block + 2;
-      }
+    if (first_segment && !from_start) {  // the block that holds the unit's last tile
+      const long long end = t + (r.tiles - cur.tile);
+      int c = static_cast<int>(min((end * shares - 1) / total, static_cast<long long>(shares - 1)));
+      while (c + 1 < shares && paged_border(total, shares, c + 1) < end) ++c;
+      while (paged_border(total, shares, c) >= end) --c;
+      parts = c - block + 2;
     }
-    if (from_start && !to_end) tail_from_start = 1, tail_slot = part;
+    if (from_start && !to_end) tail_slot = part;
     first_segment = false;
     t += tiles;
     if (t < t1) cur.next_unit(a);
   }
-  if (tid == 0) {
-    int32_t* d = p.desc + block * PA_DESC;
-    d[0] = first_mid;
-    d[1] = z_first;
-    d[2] = sub_first;
-    d[3] = parts;
-    d[4] = tail_from_start;
-    d[5] = tail_slot;
-    d[6] = first_open;
-    d[7] = 0;
-  }
+  if (tid == 0) *reinterpret_cast<int4*>(p.desc + block * PA_DESC) = make_int4(parts, z_first, sub_first, tail_slot);
 }
 
-// Joins the parts of the units that borders between blocks cut: block c takes the unit that the border
-// before block c + 1 cuts, if that is the first border in it.  With few rows several warps share a row and
-// take its parts in turn (a long request has dozens), so that few loads wait for one another.
+// Joins the parts of the units that borders between blocks cut.  The unit that block c comes in in the middle of
+// is listed for joining if block c - 1 began it.  Every block reads all descriptions, and rows of listed
+// units are dealt out: a unit of many parts (a long request has hundreds) takes a whole block a row, whose warps
+// share the parts; one of few takes a warp a row.
 constexpr int PA_JOIN_WARPS = 16;
+constexpr int PA_JOIN_MAX = 1024;  // blocks of the attention kernel
+constexpr int PA_JOIN_MANY = 16;   // parts from which on a row takes a block
+
+template <typename C>
+__device__ __forceinline__ void paged_join_store(const PagedAttnParams& p, const PagedRequest& r, int kv_head, int unit_row, int lane,
+                                                 const float2 (&v)[C::D / 64], float top, float sum) {
+  using T = typename C::type;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  const syn_paged_attn_args& a = p.a;
+  const int group = a.Hq / a.Hkv;
+  float factor = sum == 0.f ? 0.f : 1.f / sum;
+  if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
+  const int tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
+  T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+#pragma unroll
+  for (int j = 0; j < C::D / 64; ++j)
+    *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
+  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+}
 
 template <typename C>
 __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-  using T = typename C::type;
-  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int N = C::D / 64;  // pairs of columns a lane
   __shared__ float2 s_o[PA_JOIN_WARPS][C::D / 2];
   __shared__ float s_m[PA_JOIN_WARPS], s_l[PA_JOIN_WARPS];
+  __shared__ int16_t s_list[2][PA_JOIN_MAX];
+  __shared__ int s_found[2][PA_JOIN_WARPS];
   const syn_paged_attn_args& a = p.a;
-  const int c = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.Hq / a.Hkv;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 d0 = *reinterpret_cast<const int4*>(p.desc + c * PA_DESC);
-  const int2 before = *reinterpret_cast<const int2*>(p.desc + (c - 1) * PA_DESC + 4);
-  if (!d0.x || !before.x) return;
-  const int z = d0.y, sub = d0.z, parts = d0.w;
-  const PagedRequest r = paged_request<C>(a, z);
-  const int group = a.Hq / a.Hkv, kv_head = sub / r.rt, row0 = (sub - kv_head * r.rt) * C::ROWS;
-  const int rows = min(C::ROWS, r.n * group - row0);
-  int wide = 1;  // warps a row
-  while (wide * 2 * rows <= PA_JOIN_WARPS && wide * 2 <= parts) wide *= 2;
-  const int share = warp % wide;
-  auto slot = [&](int i) { return i == 0 ? before.y : 2 * (c - 1 + i); };
-  for (int first = 0; first < rows; first += PA_JOIN_WARPS / wide) {
-    const int row = first + warp / wide;
-    const bool live = row < rows;
-    float top = -CUDART_INF_F, sum = 0.f;
-    float2 v[N];
+  int count[2] = {0, 0};
+  for (int c0 = 1; c0 < p.grid; c0 += PA_JOIN_WARPS * 32) {  // in the order of the blocks: all have the same lists
+    const int c = c0 + threadIdx.x;
+    bool listed = false, many = false;
+    if (c < p.grid) {
+      const int parts = p.desc[c * PA_DESC];
+      listed = parts > 0 && p.desc[(c - 1) * PA_DESC + 3] >= 0;
+      many = parts >= PA_JOIN_MANY;
+    }
+    const unsigned mask[2] = {__ballot_sync(~0u, listed && many), __ballot_sync(~0u, listed && !many)};
+    __syncthreads();
+    if (lane < 2) s_found[lane][warp] = __popc(mask[lane]);
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
-    if (live) {
+    for (int k = 0; k < 2; ++k) {
+      int at = count[k];
+      for (int w = 0; w < PA_JOIN_WARPS; ++w) {
+        if (w < warp) at += s_found[k][w];
+        count[k] += s_found[k][w];
+      }
+      if (listed && many == (k == 0)) s_list[k][at + __popc(mask[k] & ((1u << lane) - 1))] = static_cast<int16_t>(c);
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const int wide = k == 0 ? PA_JOIN_WARPS : 1;  // warps a row
+    const int share = k == 0 ? warp : 0;
+    const int items = count[k] * C::ROWS;
+    const int from = k == 0 ? blockIdx.x : blockIdx.x * PA_JOIN_WARPS + warp;
+    const int skip = k == 0 ? gridDim.x : gridDim.x * PA_JOIN_WARPS;
+    for (int item = from; item < items; item += skip) {
+      const int c = s_list[k][item / C::ROWS], row = item % C::ROWS;
+      const int4 d = *reinterpret_cast<const int4*>(p.desc + c * PA_DESC);
+      const int before = p.desc[(c - 1) * PA_DESC + 3], parts = d.x;
+      const PagedRequest r = paged_request<C>(a, d.y);
+      const int kv_head = d.z / r.rt, row0 = (d.z - kv_head * r.rt) * C::ROWS;
+      if (row >= r.n * group - row0) continue;
+      auto slot = [&](int i) { return i == 0 ? before : 2 * (c - 1 + i); };
+      float top = -CUDART_INF_F, sum = 0.f;
+      float2 v[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
       for (int i0 = share; i0 < parts; i0 += 32 * wide) {  // a part's statistics a lane, then one part after the other
         const int i = i0 + lane * wide;
         float2 ml = make_float2(-CUDART_INF_F, 0.f);
@@ -847,49 +908,39 @@ __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __
         for (int j = 0; j < N; ++j) v[j].x *= alpha, v[j].y *= alpha;
         const int count = min(32, (parts - i0 + wide - 1) / wide);
 #pragma unroll 8
-        for (int k = 0; k < count; ++k) {
-          const float f = __shfl_sync(~0u, w, k);
-          const float* from = p.part_o + (static_cast<int64_t>(slot(i0 + k * wide)) * C::ROWS + row) * C::D + lane * 2;
+        for (int q = 0; q < count; ++q) {
+          const float f = __shfl_sync(~0u, w, q);
+          const float* at = p.part_o + (static_cast<int64_t>(slot(i0 + q * wide)) * C::ROWS + row) * C::D + lane * 2;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const float2 u = *reinterpret_cast<const float2*>(from + j * 64);
+            const float2 u = *reinterpret_cast<const float2*>(at + j * 64);
             v[j].x += u.x * f, v[j].y += u.y * f;
           }
         }
       }
-    }
-    if (wide > 1) {
-      __syncthreads();
-      if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
+      if (k == 0) {
+        __syncthreads();
+        if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
 #pragma unroll
-      for (int j = 0; j < N; ++j) s_o[warp][j * 32 + lane] = v[j];
-      __syncthreads();
-      if (live && share == 0) {
-        for (int w = 1; w < wide; ++w) top = fmaxf(top, s_m[warp + w]);
+        for (int j = 0; j < N; ++j) s_o[warp][j * 32 + lane] = v[j];
+        __syncthreads();
+        if (warp > 0) continue;
+        for (int w = 1; w < PA_JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
         const float zero = top == -CUDART_INF_F ? 0.f : top;
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
-        for (int w = 0; w < wide; ++w) {
-          const float f = ex2(s_m[warp + w] - zero);
-          sum += s_l[warp + w] * f;
+        for (int w = 0; w < PA_JOIN_WARPS; ++w) {
+          const float f = ex2(s_m[w] - zero);
+          sum += s_l[w] * f;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const float2 u = s_o[warp + w][j * 32 + lane];
+            const float2 u = s_o[w][j * 32 + lane];
             v[j].x += u.x * f, v[j].y += u.y * f;
           }
         }
       }
-    }
-    if (live && share == 0) {
-      float factor = sum == 0.f ? 0.f : 1.f / sum;
-      if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
-      const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
-      T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
-      if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
+      paged_join_store<C>(p, r, kv_head, row0 + row, lane, v, top, sum);
     }
   }
 }
