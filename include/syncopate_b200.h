@@ -568,8 +568,9 @@ typedef struct syn_paged_attn_args {
   int32_t device;
 } syn_paged_attn_args;
 int syn_paged_attention(const syn_paged_attn_args* args, void* stream);
-/* Bytes of workspace that every syn_paged_attention call on `num_sms` SMs can do with. */
-int64_t syn_paged_attention_workspace(int num_sms);
+/* Bytes of workspace that every syn_paged_attention call with head dimension D on `num_sms` SMs can do with
+ * (num_sms is not 0 here), or a negative error code. */
+int64_t syn_paged_attention_workspace(int num_sms, int D);
 
 #ifdef __cplusplus
 }

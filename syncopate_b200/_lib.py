@@ -474,7 +474,7 @@ def _declare(l: C.CDLL) -> None:
     l.syn_paged_attention.restype = C.c_int
     l.syn_paged_attention.argtypes = [C.c_char_p, C.c_void_p]
     l.syn_paged_attention_workspace.restype = C.c_int64
-    l.syn_paged_attention_workspace.argtypes = [C.c_int]
+    l.syn_paged_attention_workspace.argtypes = [C.c_int, C.c_int]
     l.syn_gemm_rs.restype = C.c_int
     l.syn_gemm_rs.argtypes = [C.POINTER(GemmRsArgs), C.POINTER(Schedule), C.POINTER(Schedule), C.c_void_p]
 

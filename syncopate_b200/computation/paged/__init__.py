@@ -25,7 +25,7 @@ from syncopate_b200 import _lib as L
 _DTYPES = {torch.float16: L.SYN_DTYPE_F16, torch.bfloat16: L.SYN_DTYPE_BF16}
 HEAD_DIMS = (64, 128, 256)
 _INT = torch.int32
-_WORKSPACE_BYTES: dict = {}  # (device, num_sms) -> bytes
+_WORKSPACE_BYTES: dict = {}  # (device, num_sms, head dimension) -> bytes
 
 
 def _refuse(where: str, what: str):
@@ -197,14 +197,14 @@ def paged_append(
         L.check(rc, "syn_paged_append")
 
 
-def _workspace(device: torch.device, num_sms: int):
-    key = (device.index, num_sms)
+def _workspace(device: torch.device, num_sms: int, dim: int):
+    key = (device.index, num_sms, dim)
     size = _WORKSPACE_BYTES.get(key)
     if size is None:
         sms = num_sms or torch.cuda.get_device_properties(device).multi_processor_count
-        size = _WORKSPACE_BYTES[key] = L.lib().syn_paged_attention_workspace(sms)
+        size = _WORKSPACE_BYTES[key] = L.lib().syn_paged_attention_workspace(sms, dim)
     # From torch's allocator at every call: calls on different streams and captured graphs never share it.
-    return (torch.empty(size, dtype=torch.uint8, device=device), size) if size else (None, 0)
+    return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def paged_attention(
@@ -295,11 +295,11 @@ def paged_attention(
     os_ = out.stride()
     cs = k_cache.stride()
     index = device.index
-    workspace, size = _workspace(device, num_sms)
+    workspace, size = _workspace(device, num_sms, dim)
     args = L.pack_paged_attn(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),
         0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), ksp, vsp,
-        0 if workspace is None else workspace.data_ptr(), size, _check_status(where, device, status), qs[0], qs[1],
+        workspace.data_ptr(), size, _check_status(where, device, status), qs[0], qs[1],
         os_[0], os_[1], cs[0], cs[1], cs[2], table_stride, sm_scale, tokens, requests, q_heads, heads, dim, page,
         pages, width, 1 if causal else 0, window, _DTYPES[dtype], code, num_sms, index)
     rc = L.lib().syn_paged_attention(args, _stream(index, None))

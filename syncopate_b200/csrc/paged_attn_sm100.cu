@@ -5,12 +5,23 @@
 
 namespace syn {
 
-// Most rows, and rows x D, of the units of an SM's resident blocks, over all variants.
-constexpr int PA_MAX_ROWS = 64;
-constexpr int PA_MAX_SIZE = 64 * 128;
+template <typename C>
+constexpr int64_t paged_worker_bytes() {
+  return PA_DESC * 4 + 2 * (C::ROWS * 2 + C::ROWS * C::D) * 4;
+}
 
-static int64_t paged_workspace(int sms) {
-  return static_cast<int64_t>(sms) * (PA_MAX_BLOCKS * PA_DESC + 2 * (PA_MAX_ROWS * 2 + PA_MAX_SIZE)) * 4;
+// Enough for every variant of head dimension D.
+static int64_t paged_workspace(int sms, int D) {
+  using T = __half;
+  auto most = [](int64_t a, int64_t b, int64_t c) { return a > b ? (a > c ? a : c) : b > c ? b : c; };
+  auto size = [](auto cfg) {
+    using C = decltype(cfg);
+    return C::BLOCKS * PA_WARPS * paged_worker_bytes<C>();
+  };
+  const int64_t bytes = D == 256   ? most(size(PagedCfg<T, false, 256, 1>()), size(PagedCfg<T, false, 256, 2>()), 0)
+                        : D == 128 ? most(size(PagedCfg<T, false, 128, 1>()), size(PagedCfg<T, false, 128, 2>()), size(PagedCfg<T, false, 128, 4>()))
+                                   : most(size(PagedCfg<T, false, 64, 1>()), size(PagedCfg<T, false, 64, 2>()), size(PagedCfg<T, false, 64, 4>()));
+  return sms * bytes;
 }
 
 // Opts the kernel into its shared memory, once a device.
@@ -30,14 +41,16 @@ static int configure_paged() {
 
 template <typename C>
 static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stream) {
-  static_assert(C::BLOCKS <= PA_MAX_BLOCKS && C::BLOCKS * C::ROWS <= PA_MAX_ROWS && C::BLOCKS * C::ROWS * C::D <= PA_MAX_SIZE,
-                "workspace");
+  // The variants for 8-bit caches have the blocks and units of those that paged_workspace counts.
+  using Counted = PagedCfg<__half, false, C::D, C::RT>;
+  static_assert(C::BLOCKS == Counted::BLOCKS && paged_worker_bytes<C>() == paged_worker_bytes<Counted>(), "workspace");
   int rc = configure_paged<C>();
   if (rc != SYN_OK) return rc;
   PagedAttnParams p;
   p.a = a;
-  p.grid = sms * C::BLOCKS < PA_JOIN_MAX ? sms * C::BLOCKS : PA_JOIN_MAX;
-  p.min_tiles = 4;
+  const int grid = sms * C::BLOCKS;
+  p.workers = grid * PA_WARPS;
+  p.min_steps = 4;
   // mulhi(n, 2^(31 + b) / d rounded up) >> (b - 1) = n / d for 0 <= n < 2^31, 2^(b - 1) < d <= 2^b
   p.page_mul = 0, p.page_shift = 0;
   if (a.page_size > 1) {
@@ -47,17 +60,16 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
     p.page_shift = b - 1;
   }
   p.desc = static_cast<int32_t*>(a.workspace);
-  p.part_ml = reinterpret_cast<float*>(p.desc + p.grid * PA_DESC);
-  p.part_o = p.part_ml + static_cast<int64_t>(2) * p.grid * C::ROWS * 2;
-  paged_attn_kernel<C><<<p.grid, PA_THREADS, C::SMEM, stream>>>(p);
+  p.part_ml = reinterpret_cast<float*>(p.desc + p.workers * PA_DESC);
+  p.part_o = p.part_ml + static_cast<int64_t>(2) * p.workers * C::ROWS * 2;
+  paged_attn_kernel<C><<<grid, PA_THREADS, C::SMEM, stream>>>(p);
   SYN_CUDA_TRY(cudaGetLastError());
-  if (p.grid < 2) return SYN_OK;
   // The join's blocks are brought in while the last shares are still at work and wait for them there.
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(sms);
+  config.gridDim = dim3((p.workers - 2) / PA_JOIN_WARPS + 1, PagedJoinCfg<C>::SLICES);
   config.blockDim = dim3(PA_JOIN_WARPS * 32);
   config.stream = stream;
   config.attrs = &attr;
@@ -108,8 +120,10 @@ int preload_paged_attn_kernels() {
 
 }  // namespace syn
 
-extern "C" int64_t syn_paged_attention_workspace(int num_sms) {
-  return num_sms <= 0 ? SYN_ERR_INVALID : syn::paged_workspace(num_sms);
+extern "C" int64_t syn_paged_attention_workspace(int num_sms, int D) {
+  if (num_sms <= 0) return SYN_ERR_INVALID;
+  if (D != 64 && D != 128 && D != 256) return SYN_ERR_UNSUPPORTED;
+  return syn::paged_workspace(num_sms, D);
 }
 
 extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
@@ -142,7 +156,7 @@ extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
   const int rc = device_sm_count(&sms);
   if (rc != SYN_OK) return rc;
   if (a->num_sms > 0 && a->num_sms < sms) sms = a->num_sms;
-  if (a->workspace == nullptr || a->workspace_bytes < paged_workspace(sms)) return SYN_ERR_INVALID;
+  if (a->workspace == nullptr || a->workspace_bytes < paged_workspace(sms, a->D)) return SYN_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == SYN_DTYPE_BF16) {
     return e4m3 ? launch_paged<__nv_bfloat16, true>(p, sms, s) : launch_paged<__nv_bfloat16, false>(p, sms, s);

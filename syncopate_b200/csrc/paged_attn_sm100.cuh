@@ -10,13 +10,12 @@
 // are small ones on mma.sync, whose fragments stay in registers; they are turned round (keys by rows,
 // dimensions by rows) because rows then come in eights, as groups do, and not in sixteens.  The layout is chosen
 // for loads in flight:
-//   * Every warp streams keys of its own through a ring of its own in shared memory (cp.async of 16
-//     bytes, a page lookup per key), so no barrier stands between loading and computing; the warps of a
-//     block meet only when a unit of rows ends.
-//   * The work (requests x key-value heads x row tiles x key tiles) is laid out in one line and cut into
-//     equal shares for a grid that fills the GPU, whatever the lengths; loads run on across the borders of
-//     units.  A unit that a border cuts leaves partial results, which a second small kernel joins in a fixed
-//     order: results do not depend on timing, there are no atomics and no state between calls.
+//   * Every warp is a worker of its own: it streams its keys and values through a ring of its own in shared memory
+//     (cp.async of 16 bytes, a page lookup a step), with no barrier between the warps of a block.
+//   * The work (requests x key-value heads x row tiles x steps of keys) is laid out in one line and cut into
+//     equal shares for the warps of a grid that fills the GPU, whatever the lengths; loads run on across the
+//     borders of units.  A unit that a border cuts leaves partial results, which a second small kernel joins
+//     in a fixed order: results do not depend on timing, there are no atomics and no state between calls.
 #pragma once
 #include <math_constants.h>
 
@@ -28,21 +27,20 @@ namespace syn {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
-constexpr int PA_MAX_BLOCKS = 3;  // resident blocks an SM, over all variants
 // The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
 // than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
 constexpr float PA_SLACK = 8.f;
-constexpr int PA_DESC = 4;  // int32 words a block leaves for the join
+constexpr int PA_DESC = 8;  // int32 words a worker leaves for the join
 
 struct PagedAttnParams {
   syn_paged_attn_args a;
-  int32_t grid;       // blocks of the launch
-  int32_t min_tiles;  // fewest key tiles worth a block
+  int32_t workers;    // warps of the launch
+  int32_t min_steps;  // fewest steps worth a worker
   uint32_t page_mul;  // key / page_size = mulhi(key, page_mul) >> page_shift (page_mul 0: pages of one key)
   int32_t page_shift;
-  float* part_o;      // [2 * grid][rows of a unit][D]
-  float* part_ml;     // [2 * grid][rows of a unit][2]
-  int32_t* desc;      // [grid][PA_DESC]
+  float* part_o;      // [2 * workers][fragments of the output: D / 16, 8-row tiles][lanes][4]
+  float* part_ml;     // [2 * workers][rows of a unit][2]
+  int32_t* desc;      // [workers][PA_DESC]
 };
 
 template <typename T, bool E4M3_, int D_, int RT_>
@@ -53,24 +51,18 @@ struct PagedCfg {
   static constexpr int RT = RT_;                     // 8-row tiles of a unit
   static constexpr int ROWS = 8 * RT;
   static constexpr int KEYS = E4M3 ? 32 : 16;        // keys of a warp's step
-  static constexpr int TILE = KEYS * PA_WARPS;       // keys of a block's step
   static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
   static constexpr int HALFB = KEYS * ROWB;          // the keys of a step, or its values
   static constexpr int BLOCKS = D == 256 ? 3 - RT : RT <= 2 ? 3 : 2;  // resident on an SM
-  static constexpr int SLOTS = (D == 256 ? 24 : RT <= 2 ? 16 : 20) * 1024 / HALFB;
+  static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? (RT <= 2 ? 4 : 5) : (RT <= 2 ? 8 : 10);
   static constexpr int RING = SLOTS * HALFB;         // bytes a warp
   static constexpr bool QREG = RT * D <= 256;        // query fragments in registers, else in shared memory
   static constexpr int KSTEPS = D / 16;
   static constexpr int DT = D / 16;                  // 16-dimension tiles of the output
-  static constexpr int DC = RT == 4 ? 16 : 32;  // output dimensions of a merge pass
-  static constexpr int NT_PASS = DC / 8;
-  static constexpr int PASSES = D / DC;
-  static constexpr int MERGE_LD = DC + 4;
-  static constexpr int SMEM_Q = QREG ? 0 : KSTEPS * RT * 256;
-  static constexpr int SMEM_MERGE = PA_WARPS * ROWS * MERGE_LD * 4;
-  static constexpr int SMEM_ML = PA_WARPS * ROWS * 2 * 4;
-  static constexpr int SMEM = PA_WARPS * RING + SMEM_Q + SMEM_MERGE + SMEM_ML;
+  static constexpr int FRAGS = DT * RT;              // output fragments of a unit, four numbers a lane
+  static constexpr int QB = QREG ? 0 : KSTEPS * RT * 256;
+  static constexpr int SMEM = PA_WARPS * (RING + QB);
   static_assert(BLOCKS * (SMEM + 1280) <= 228 * 1024, "shared memory of an SM");
   static_assert(SLOTS >= 3, "a key half, a value half and one on its way");
 };
@@ -161,7 +153,7 @@ struct PagedRequest {
   int s0, n;       // rows of q: first one, how many
   int len;         // keys (one more than the table has room for, where the length says more)
   int first;       // first key that any row sees
-  int tiles, rt;   // key tiles of a unit; row tiles a head
+  int steps, rt;   // steps of a unit; row tiles a head
 };
 
 template <typename C>
@@ -177,28 +169,28 @@ __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args&
   if (len > room) len = static_cast<int>(min(room + 1, static_cast<long long>(INT_MAX)));
   r.len = len;
   r.first = a.window > 0 ? max(0, min(len, len - r.n - a.window + 1)) : 0;
-  r.tiles = max(1, (len - r.first + C::TILE - 1) / C::TILE);
+  r.steps = max(1, (len - r.first + C::KEYS - 1) / C::KEYS);
   r.rt = (r.n * (a.Hq / a.Hkv) + C::ROWS - 1) / C::ROWS;
   return r;
 }
 
 __device__ __forceinline__ long long paged_border(long long total, int shares, int c) { return total * c / shares; }
 
-// Position on the line: key tile `tile` of unit `sub` (head * row tiles + row tile) of request z.
+// Position on the line: step `step` of unit `sub` (head * row tiles + row tile) of request z.
 template <typename C>
 struct PagedCursor {
-  int z, sub, tile;
+  int z, sub, step;
   PagedRequest r;
 
   __device__ __forceinline__ void at(const syn_paged_attn_args& a, int z_, long long rest) {
     z = z_;
     r = paged_request<C>(a, z);
-    sub = static_cast<int>(rest / r.tiles);
-    tile = static_cast<int>(rest % r.tiles);
+    sub = static_cast<int>(rest / r.steps);
+    step = static_cast<int>(rest % r.steps);
   }
-  // To the first tile of the next unit; the caller knows that there is one.
+  // To the first step of the next unit; the caller knows that there is one.
   __device__ __forceinline__ void next_unit(const syn_paged_attn_args& a) {
-    tile = 0;
+    step = 0;
     if (++sub < a.Hkv * r.rt) return;
     sub = 0;
     do {
@@ -217,11 +209,11 @@ struct PagedCursor {
 template <typename C, typename F>
 __device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
   if constexpr (!C::E4M3) {
-    const int row = (lane & 7) + (lane >> 4) * 8;
+    const uint32_t at = v + ((lane & 7) + (lane >> 4) * 8) * C::ROWB + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
     for (int j = 0; j < C::DT; ++j) {
       uint32_t a[4];
-      ldsm4t(v + row * C::ROWB + (((j * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), a);
+      ldsm4t((at ^ (j % 4 * 32)) + j / 4 * 128, a);
       f(j, a);
     }
   } else {
@@ -259,8 +251,11 @@ __device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
   }
 }
 
-// Place of 16-byte chunk `chunk` of row `row` in a warp's ring (chosen so that the reads above and those of
-// the keys below meet no bank twice; D = 64 in 8 bits reads its values two deep).
+// Place of 16-byte chunk `chunk` of row `row` in a half of a warp's ring: chunks change places within 128 bytes
+// so that the reads above and those of the keys below meet no bank twice (D = 64 in 8 bits reads its values two
+// deep).  Halves are aligned to 128 bytes, so a change of chunk is an exclusive or with the address.  (Rows 16 bytes
+// apart instead cost the copies into shared memory more than the plainer addresses gave: 585 against 549 us on
+// 3.5 GB of 16-bit keys and values.)
 template <typename C, bool VALUES>
 __device__ __forceinline__ uint32_t ring_at(int row, int chunk) {
   int c = chunk;
@@ -269,19 +264,60 @@ __device__ __forceinline__ uint32_t ring_at(int row, int chunk) {
   else if constexpr (C::D != 64) c ^= (row & 1) << 2;
   return row * C::ROWB + (c << 4);
 }
-
-// Dimension of entry e (0 .. DC - 1) of merge pass `pass`; entries 2 i and 2 i + 1 are neighbours.
-template <typename C>
-__device__ __forceinline__ int merge_dim(int pass, int e) {
-  if constexpr (!C::E4M3) return pass * C::DC + e;
-  const int nt = pass * C::NT_PASS + e % C::NT_PASS, c = e / C::NT_PASS;
-  if constexpr (C::D == 64) return 8 * c + nt;
-  return (nt / 16) * 128 + 16 * c + nt % 16;
+// The same for the chunk that lane `lane` brings in its i-th turn, row i * (32 / CPR) + lane / CPR, given its place
+// in turn 0: `own` = ring_at(lane / CPR, lane % CPR).
+template <typename C, bool VALUES>
+__device__ __forceinline__ uint32_t ring_turn(uint32_t own, int i) {
+  constexpr int RPI = 32 / C::CPR;
+  const int row = i * RPI;  // shares no bit with lane / CPR
+  int flip = 0;
+  if constexpr (!C::E4M3) flip = row & 7;
+  else if constexpr (VALUES) flip = C::D == 64 ? (row >> 1) & 3 : ((row >> 1) & 3) << 1;
+  else if constexpr (C::D != 64) flip = (row & 1) << 2;
+  return (own ^ (flip << 4)) + row * C::ROWB;
 }
-// Entry of row c of the pass's i-th 8-dimension tile.
-template <typename C>
-__device__ __forceinline__ int merge_entry(int i, int c) {
-  return C::E4M3 ? c * C::NT_PASS + i : i * 8 + c;
+
+__device__ __forceinline__ void paged_lse(const syn_paged_attn_args& a, int s0, int kv_head, int unit_row, float m, float l) {
+  const int group = a.Hq / a.Hkv, tok = unit_row / group;
+  if (a.lse != nullptr) a.lse[static_cast<int64_t>(s0 + tok) * a.Hq + kv_head * group + unit_row - tok * group] = m + log2f(l);
+}
+
+// Writes rows (8 rows of tile j, those below `rows`) of COUNT output fragments from fragment tile `dt` on, which hold
+// dimensions by rows, times `factor` of the lane's two rows.
+template <typename C, int COUNT>
+__device__ __forceinline__ void store_frags(const syn_paged_attn_args& a, const float (&o)[COUNT][4], int dt, const float (&factor)[2],
+                                            int s0, int kv_head, int unit_row, int rows, int lane) {
+  using T = typename C::type;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  const int g = lane >> 2, t4 = lane & 3, group = a.Hq / a.Hkv;
+  auto out_row = [&](int row) {
+    const int tok = (unit_row + row) / group, head = kv_head * group + unit_row + row - tok * group;
+    return static_cast<T*>(a.o) + static_cast<int64_t>(s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+  };
+  if constexpr (!C::E4M3) {  // turned back 8 x 8: lane (g, t4) then has dimensions 2 t4, 2 t4 + 1 of row g
+    T* out = out_row(min(g, rows - 1)) + dt * 16 + 2 * t4;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const uint32_t x = transpose8(pack2<BF16>(o[i][0] * factor[0], o[i][1] * factor[1]));
+      const uint32_t y = transpose8(pack2<BF16>(o[i][2] * factor[0], o[i][3] * factor[1]));
+      if (g < rows) {
+        *reinterpret_cast<uint32_t*>(out + i * 16) = x;
+        *reinterpret_cast<uint32_t*>(out + i * 16 + 8) = y;
+      }
+    }
+  } else {  // the halves of a fragment are neighbours
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (2 * t4 + c < rows) {
+        T* out = out_row(2 * t4 + c);
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+          const int nt = 2 * (dt + i), d = C::D == 64 ? 8 * g + nt : (nt / 16) * 128 + 16 * g + nt % 16;
+          *reinterpret_cast<uint32_t*>(out + d) = pack2<BF16>(o[i][c] * factor[c], o[i][2 + c] * factor[c]);
+        }
+      }
+    }
+  }
 }
 
 template <typename C>
@@ -291,21 +327,20 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   constexpr bool MBF16 = BF16 && !C::E4M3;  // type of the matrix products: 8-bit values are halves there
   constexpr int RT = C::RT;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_sum[PA_WARPS];
-  __shared__ long long s_rest;
-  __shared__ int s_z;
+  __shared__ long long s_sum[PA_WARPS], s_rest[PA_WARPS];
+  __shared__ int s_z[PA_WARPS];
   const syn_paged_attn_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int group = a.Hq / a.Hkv;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this block's share of the line
+  // ---- this warp's share of the line
   const int per = (a.requests + PA_THREADS - 1) / PA_THREADS;
   const int z0 = min(tid * per, a.requests), z1 = min(z0 + per, a.requests);
   long long mine = 0;
   for (int z = z0; z < z1; ++z) {
     const PagedRequest r = paged_request<C>(a, z);
-    mine += static_cast<long long>(r.tiles) * a.Hkv * r.rt;
+    mine += static_cast<long long>(r.steps) * a.Hkv * r.rt;
     if (blockIdx.x == 0) {
       if (a.lens[z] < 0) paged_record(a.status, SYN_DEV_BAD_INDEX, z, a.lens[z]);
       if (a.starts != nullptr && (a.starts[z] < 0 || a.starts[z + 1] < a.starts[z] || a.starts[z + 1] > a.tokens))
@@ -324,42 +359,48 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     if (w < warp) upto += s_sum[w];
     total += s_sum[w];
   }
-  const int shares = static_cast<int>(min(static_cast<long long>(p.grid), max(1LL, total / p.min_tiles)));
-  const int block = blockIdx.x;
-  const long long t0 = block < shares ? paged_border(total, shares, block) : total;
-  const long long t1 = block < shares ? paged_border(total, shares, block + 1) : total;
+  const int shares = static_cast<int>(min(static_cast<long long>(p.workers), max(1LL, total / p.min_steps)));
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {  // neighbouring shares go to different blocks
+    const int share = w * gridDim.x + blockIdx.x;
+    const long long from = share < shares ? paged_border(total, shares, share) : total;
+    if (upto - mine <= from && from < upto) {
+      long long rest = from - (upto - mine);
+      int z = z0;
+      for (; z < z1; ++z) {
+        const PagedRequest r = paged_request<C>(a, z);
+        const long long n = static_cast<long long>(r.steps) * a.Hkv * r.rt;
+        if (rest < n) break;
+        rest -= n;
+      }
+      s_z[w] = z;
+      s_rest[w] = rest;
+    }
+  }
+  __syncthreads();  // the last barrier: from here on the warps go their own ways
+  const int worker = warp * gridDim.x + blockIdx.x;
+  int32_t* desc = p.desc + worker * PA_DESC;
+  const long long t0 = worker < shares ? paged_border(total, shares, worker) : total;
+  const long long t1 = worker < shares ? paged_border(total, shares, worker + 1) : total;
   if (t0 >= t1) {
-    if (tid == 0) *reinterpret_cast<int4*>(p.desc + block * PA_DESC) = make_int4(0, 0, 0, -1);
+    if (lane == 0) *reinterpret_cast<int4*>(desc) = make_int4(0, -1, 0, 0);
     return;
   }
-  if (upto - mine <= t0 && t0 < upto) {
-    long long rest = t0 - (upto - mine);
-    int z = z0;
-    for (; z < z1; ++z) {
-      const PagedRequest r = paged_request<C>(a, z);
-      const long long w = static_cast<long long>(r.tiles) * a.Hkv * r.rt;
-      if (rest < w) break;
-      rest -= w;
-    }
-    s_z = z;
-    s_rest = rest;
-  }
-  __syncthreads();
 
   PagedCursor<C> cur;
-  cur.at(a, s_z, s_rest);
+  cur.at(a, s_z[warp], s_rest[warp]);
 
   // ---- producer: halves of steps (keys, values, keys, ...) are asked for SLOTS - 1 halves ahead, across units
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   PagedCursor<C> ahead = cur;
-  long long t_ahead = t0;
+  int left = static_cast<int>(t1 - t0);  // steps that are yet to be asked for
   int page = -2, inside = 0;  // page of key (lane % KEYS) of the next step (-2: no such key), slot in it
   int head_ahead = ahead.sub / ahead.r.rt;
-  constexpr int EB = C::E4M3 ? 1 : 2, RPI = 32 / C::CPR == 0 ? 1 : 32 / C::CPR, LOADS = C::HALFB / 512;
+  constexpr int EB = C::E4M3 ? 1 : 2, RPI = 32 / C::CPR, LOADS = C::KEYS / RPI;
   auto look_up = [&]() {
     page = -2;
-    if (t_ahead < t1) {
-      const int key = ahead.r.first + ahead.tile * C::TILE + warp * C::KEYS + (lane & (C::KEYS - 1));
+    if (left > 0) {
+      const int key = ahead.r.first + ahead.step * C::KEYS + (lane & (C::KEYS - 1));
       if (key < ahead.r.len) {
         const int i = p.page_mul ? __umulhi(key, p.page_mul) >> p.page_shift : key;
         inside = key - i * a.page_size;
@@ -370,7 +411,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   long long off = -2;     // byte offset of this lane's key in the caches (-2: no such key, -1: no such page)
   bool one_page = false;  // the step's keys lie behind one another in one page, all of them there
   auto issue = [&](uint32_t slot, bool values) {
-    if (t_ahead < t1) {
+    if (left > 0) {
       if (!values) {
         off = -2;
         if (page != -2) {
@@ -390,16 +431,16 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       if (one_page) {
         const char* from = base + off;
         const int64_t skip = RPI * a.cache_strides[1] * EB;
+        const uint32_t own = slot + (values ? ring_at<C, true>(lane / C::CPR, lane % C::CPR) : ring_at<C, false>(lane / C::CPR, lane % C::CPR));
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-          const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
-          cp_async16(slot + (values ? ring_at<C, true>(row, chunk) : ring_at<C, false>(row, chunk)), from);
+          cp_async16(values ? ring_turn<C, true>(own, i) : ring_turn<C, false>(own, i), from);
           from += skip;
         }
       } else {
 #pragma unroll 2
         for (int i = 0; i < LOADS; ++i) {
-          const int row = (i * 32 + lane) / C::CPR, chunk = (i * 32 + lane) % C::CPR;
+          const int row = i * RPI + lane / C::CPR, chunk = lane % C::CPR;
           const long long o = __shfl_sync(~0u, off, row);
           const uint32_t to = slot + (values ? ring_at<C, true>(row, chunk) : ring_at<C, false>(row, chunk));
           if (o == -1) sts16(to, ~0u, ~0u, ~0u, ~0u);  // no such page: NaN in every type
@@ -408,9 +449,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         }
       }
       if (values) {
-        ++t_ahead;
-        if (++ahead.tile == ahead.r.tiles) {
-          if (t_ahead < t1) ahead.next_unit(a);
+        --left;
+        if (++ahead.step == ahead.r.steps) {
+          if (left > 0) ahead.next_unit(a);
           head_ahead = ahead.sub / ahead.r.rt;
         }
         look_up();
@@ -423,23 +464,20 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   for (int s = 0; s < C::SLOTS - 1; ++s) issue(ring + s * C::HALFB, s & 1);
   // Slot of the half being read; the one read before it is the next to fill.
   int slot = 0;
-  auto next_half = [&](bool values) {
+  auto ready = [&]() {
     cp_async_wait<C::SLOTS - 2>();
     __syncwarp();
-    const uint32_t at = ring + slot * C::HALFB;
+    return ring + slot * C::HALFB;
+  };
+  auto refill = [&](bool values) {  // `values`: what the half being read holds
     issue(ring + (slot == 0 ? C::SLOTS - 1 : slot - 1) * C::HALFB, (C::SLOTS & 1) ? values : !values);
     if (++slot == C::SLOTS) slot = 0;
-    return at;
   };
 
-  const uint32_t q_smem = smem_u32(smem) + PA_WARPS * C::RING;
-  float* merge = reinterpret_cast<float*>(smem + PA_WARPS * C::RING + C::SMEM_Q);
-  float* s_m = merge + C::SMEM_MERGE / 4;  // [warp][row]
-  float* s_l = s_m + PA_WARPS * C::ROWS;
+  const uint32_t q_smem = smem_u32(smem) + PA_WARPS * C::RING + warp * C::QB;
   long long t = t0;
-  int parts = 0;       // of the unit that this block comes in in the middle of, from the block before on
-  int tail_slot = -1;  // part of the unit that it begins and does not end
-  const int z_first = cur.z, sub_first = cur.sub;
+  int tail_slot = -1;  // part of the unit that this worker begins and does not end
+  int4 mid0 = make_int4(0, 0, 0, 0), mid1 = mid0;  // the unit that it comes in in the middle of
   bool first_segment = true;
 
   while (t < t1) {
@@ -448,7 +486,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const int kv_head = cur.sub / r.rt, row0 = (cur.sub - kv_head * r.rt) * C::ROWS;
     const int rows = min(C::ROWS, r.n * group - row0);
     const int pos0 = r.len - r.n;
-    const int tiles = static_cast<int>(min(static_cast<long long>(r.tiles - cur.tile), t1 - t));
+    const int steps = static_cast<int>(min(static_cast<long long>(r.steps - cur.step), t1 - t));
     // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
     // Rows behind the last repeat it.
     int lo[2 * RT], hi[2 * RT];
@@ -515,9 +553,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
         for (int i = 0; i < RT; ++i) q_frag(ks, i, qreg[ks * RT + i]);
     } else {
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < C::KSTEPS / PA_WARPS; ++j) {
-        const int ks = j * PA_WARPS + warp;
+      for (int ks = 0; ks < C::KSTEPS; ++ks)
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           uint32_t f[2];
@@ -525,8 +563,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
           asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(q_smem + (ks * RT + i) * 256 + lane * 8), "r"(f[0]), "r"(f[1])
                        : "memory");
         }
-      }
-      __syncthreads();
+      __syncwarp();
     }
     auto q_at = [&](int ks, int i, uint32_t (&f)[2]) {
       if constexpr (C::QREG) {
@@ -537,9 +574,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       }
     };
 
-    float o[C::DT][RT][4], m[2 * RT], l[2 * RT];
+    float o[C::DT][RT][4], m[2 * RT], slack[2 * RT], l[2 * RT];
 #pragma unroll
-    for (int x = 0; x < 2 * RT; ++x) m[x] = -CUDART_INF_F, l[x] = 0.f;
+    for (int x = 0; x < 2 * RT; ++x) m[x] = 0.f, slack[x] = -CUDART_INF_F, l[x] = 0.f;  // slack: the reference may stay that far behind
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
@@ -547,11 +584,13 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[dt][i][c] = 0.f;
 
-    for (int i = 0; i < tiles; ++i) {
-      const uint32_t k_at = next_half(false);
-      const int base = r.first + (cur.tile + i) * C::TILE + warp * C::KEYS;
-      if (base >= r.len) {  // no key of this warp
-        next_half(true);
+    for (int i = 0; i < steps; ++i) {
+      const int base = r.first + (cur.step + i) * C::KEYS;
+      const uint32_t k_at = ready();
+      if (base >= r.len) {  // no key at all
+        refill(false);
+        ready();
+        refill(true);
         continue;
       }
 
@@ -565,18 +604,33 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
           for (int c = 0; c < 4; ++c) s[n][j][c] = 0.f;
       if constexpr (!C::E4M3) {
-        const int row = lane & 15;
+        const uint32_t at = k_at + (lane & 15) * C::ROWB + (((lane >> 4) ^ (lane & 7)) << 4);
+        float s2[RT][4];  // two sums, so that a product waits for the last but one
 #pragma unroll
-        for (int ks = 0; ks < C::KSTEPS; ++ks) {
-          uint32_t k[4];
-          ldsm4(k_at + row * C::ROWB + (((ks * 2 + (lane >> 4)) ^ (row & 7)) << 4), k);
+        for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int j = 0; j < RT; ++j) {
-            uint32_t f[2];
-            q_at(ks, j, f);
-            mma16816<MBF16>(s[0][j], k, f[0], f[1]);
-          }
+          for (int c = 0; c < 4; ++c) s2[j][c] = 0.f;
+        constexpr int GROUP = C::KSTEPS < 8 ? C::KSTEPS : 8;
+#pragma unroll
+        for (int k0 = 0; k0 < C::KSTEPS; k0 += GROUP) {
+          uint32_t k[GROUP][4];
+#pragma unroll
+          for (int ks = 0; ks < GROUP; ++ks) ldsm4((at ^ ((k0 + ks) % 4 * 32)) + (k0 + ks) / 4 * 128, k[ks]);
+          if (k0 == 0) refill(false);  // its arithmetic fills the wait for the fragments
+#pragma unroll
+          for (int ks = 0; ks < GROUP; ++ks)
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+              uint32_t f[2];
+              q_at(k0 + ks, j, f);
+              if (ks & 1) mma16816<MBF16>(s2[j], k[ks], f[0], f[1]);
+              else mma16816<MBF16>(s[0][j], k[ks], f[0], f[1]);
+            }
         }
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[0][j][c] += s2[j][c];
       } else {
 #pragma unroll
         for (int part = 0; part < C::D / 64; ++part) {
@@ -587,8 +641,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
             for (int j = 0; j < RT; ++j) q_at(part * 4 + w, j, f[w][j]);
 #pragma unroll
           for (int n = 0; n < SN; ++n) {
-            const uint4 x = lds16(k_at + ring_at<C, false>(n * 16 + g, t4 + part * 4));
-            const uint4 y = lds16(k_at + ring_at<C, false>(n * 16 + 8 + g, t4 + part * 4));
+            const uint32_t at = k_at + ring_at<C, false>(g, t4 + part * 4) + n * 16 * C::ROWB;
+            const uint4 x = lds16(at), y = lds16(at + 8 * C::ROWB);
+            if (part == 0 && n == 0) refill(false);  // its arithmetic fills the wait for the keys
             const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -604,6 +659,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
       // ---- weights
       const bool whole = base >= all_lo && base + C::KEYS <= all_hi;  // every row sees every key
+      float y[SN][RT][4];  // score minus reference, in powers of two
       bool rise = false;
 #pragma unroll
       for (int x = 0; x < 2 * RT; ++x)
@@ -611,44 +667,51 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float& v = s[n][x >> 1][2 * h + (x & 1)];
-            v *= mult[x];
-            const int key = base + n * 16 + h * 8 + g;
+            const int c = 2 * h + (x & 1), key = base + n * 16 + h * 8 + g;
+            float& v = y[n][x >> 1][c];
+            v = fmaf(s[n][x >> 1][c], mult[x], -m[x]);
             if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
-            rise |= v > m[x] + PA_SLACK;
+            rise |= v > slack[x];
           }
       if (__any_sync(~0u, rise)) {
 #pragma unroll
         for (int x = 0; x < 2 * RT; ++x) {
-          float top = m[x];
+          float top = -CUDART_INF_F;
 #pragma unroll
-          for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[n][x >> 1][x & 1], s[n][x >> 1][2 + (x & 1)]));
+          for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(y[n][x >> 1][x & 1], y[n][x >> 1][2 + (x & 1)]));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-          const float alpha = ex2(m[x] - (top == -CUDART_INF_F ? 0.f : top));
-          m[x] = top;
-          l[x] *= alpha;
+          const bool none = slack[x] == -CUDART_INF_F;  // no key so far: any reference will do
+          if (top > (none ? -CUDART_INF_F : 0.f)) {
+            const float by = m[x] + top - m[x], alpha = none ? 0.f : ex2(-by);
+            m[x] += top;
+            slack[x] = PA_SLACK;
+            l[x] *= alpha;
 #pragma unroll
-          for (int dt = 0; dt < C::DT; ++dt) {
-            o[dt][x >> 1][x & 1] *= alpha;
-            o[dt][x >> 1][2 + (x & 1)] *= alpha;
+            for (int dt = 0; dt < C::DT; ++dt) {
+              o[dt][x >> 1][x & 1] *= alpha;
+              o[dt][x >> 1][2 + (x & 1)] *= alpha;
+            }
+#pragma unroll
+            for (int n = 0; n < SN; ++n)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) y[n][x >> 1][2 * h + (x & 1)] -= by;
           }
         }
       }
 #pragma unroll
-      for (int x = 0; x < 2 * RT; ++x) {
-        const float zero = m[x] == -CUDART_INF_F ? 0.f : m[x];
+      for (int x = 0; x < 2 * RT; ++x)
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float& v = s[n][x >> 1][2 * h + (x & 1)];
-            v = ex2(v - zero);
+            float& v = y[n][x >> 1][2 * h + (x & 1)];
+            v = ex2(v);
             l[x] += v;
           }
-      }
-      const uint32_t v_at = next_half(true);
+      const uint32_t v_at = ready();
+      refill(true);
 
       // ---- values, transposed: 16 dimensions by 8 rows a product.  The weights enter as two 16-bit numbers, the
       // second one what the first left, so that their rounding does not add to that of the output.
@@ -659,11 +722,11 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int j = 0; j < RT; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float x = s[kk][j][2 * h], y = s[kk][j][2 * h + 1];
-            const uint32_t top = pack2<MBF16>(x, y);
+            const float w0 = y[kk][j][2 * h], w1 = y[kk][j][2 * h + 1];
+            const uint32_t top = pack2<MBF16>(w0, w1);
             ph[j][h] = transpose8(top);
             const float2 b = unpack2<MBF16>(top);
-            pl[j][h] = transpose8(pack2<MBF16>(x - b.x, y - b.y));
+            pl[j][h] = transpose8(pack2<MBF16>(w0 - b.x, w1 - b.y));
           }
         bool odd = false;  // values that are not finite, at keys that not every row sees
         if (!whole && r.n > 1) {
@@ -712,236 +775,185 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       }
     }
 
-    // ---- the warps' parts of the unit are put together
+    // ---- the unit, or this worker's part of it, is done
+    const bool from_start = cur.step == 0, to_end = cur.step + steps == r.steps, partial = !(from_start && to_end);
+    const int part = 2 * worker + (first_segment ? 0 : 1);
 #pragma unroll
     for (int x = 0; x < 2 * RT; ++x) {
       l[x] += __shfl_xor_sync(~0u, l[x], 4);
       l[x] += __shfl_xor_sync(~0u, l[x], 8);
       l[x] += __shfl_xor_sync(~0u, l[x], 16);
-      const int row = (x >> 1) * 8 + 2 * t4 + (x & 1);
-      if (g == 0) s_m[warp * C::ROWS + row] = m[x], s_l[warp * C::ROWS + row] = l[x];
+      if (slack[x] == -CUDART_INF_F) m[x] = -CUDART_INF_F;
     }
-    __syncthreads();
+    if (partial) {
+      float4* to = reinterpret_cast<float4*>(p.part_o) + static_cast<int64_t>(part) * C::FRAGS * 32 + lane;
 #pragma unroll
-    for (int x = 0; x < 2 * RT; ++x) {
-      const int row = (x >> 1) * 8 + 2 * t4 + (x & 1);
-      float top = -CUDART_INF_F;
+      for (int j = 0; j < RT; ++j)
+        if (j * 8 + 2 * t4 < rows) {
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + row]);
-      const float f = ex2(m[x] - (top == -CUDART_INF_F ? 0.f : top));
-#pragma unroll
-      for (int dt = 0; dt < C::DT; ++dt) {
-        o[dt][x >> 1][x & 1] *= f;
-        o[dt][x >> 1][2 + (x & 1)] *= f;
-      }
-    }
-    constexpr int TPR = C::DC / 4;  // threads a row
-    static_assert(C::ROWS * TPR <= PA_THREADS, "a thread for every four outputs of a pass");
-    const bool writer = tid < C::ROWS * TPR;
-    const int row = writer ? tid / TPR : 0, entry = (tid % TPR) * 4;
-    float top = -CUDART_INF_F, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, s_m[w * C::ROWS + row]);
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) sum += s_l[w * C::ROWS + row] * ex2(s_m[w * C::ROWS + row] - (top == -CUDART_INF_F ? 0.f : top));
-    const bool from_start = cur.tile == 0, to_end = cur.tile + tiles == r.tiles, partial = !(from_start && to_end);
-    const int part = 2 * block + (first_segment ? 0 : 1);
-    const int unit_row = row0 + row, tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
-    float factor = 1.f;
-    if (!partial) {
-      factor = sum == 0.f ? 0.f : 1.f / sum;
-      if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
-    }
-    if (writer && row < rows && entry == 0) {
-      if (partial) {
-        p.part_ml[(part * C::ROWS + row) * 2] = top;
-        p.part_ml[(part * C::ROWS + row) * 2 + 1] = sum;
-      } else if (a.lse != nullptr) {
-        a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
-      }
-    }
-    T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
-    float* out_part = p.part_o + (static_cast<int64_t>(part) * C::ROWS + row) * C::D;
-#pragma unroll
-    for (int pass = 0; pass < C::PASSES; ++pass) {
-      if (pass > 0) __syncthreads();
-#pragma unroll
-      for (int x = 0; x < 2 * RT; ++x) {
-        const int to_row = (x >> 1) * 8 + 2 * t4 + (x & 1);
-        if (to_row < rows) {
-          float* to = merge + (warp * C::ROWS + to_row) * C::MERGE_LD;
-#pragma unroll
-          for (int n = 0; n < C::NT_PASS; ++n) {
-            const int nt = pass * C::NT_PASS + n;
-            to[merge_entry<C>(n, g)] = o[nt >> 1][x >> 1][2 * (nt & 1) + (x & 1)];
-          }
+          for (int dt = 0; dt < C::DT; ++dt)
+            to[(dt * RT + j) * 32] = make_float4(o[dt][j][0], o[dt][j][1], o[dt][j][2], o[dt][j][3]);
+          if (g == 0)
+            *reinterpret_cast<float4*>(p.part_ml + (static_cast<int64_t>(part) * C::ROWS + j * 8 + 2 * t4) * 2) =
+                make_float4(m[2 * j], l[2 * j], m[2 * j + 1], l[2 * j + 1]);
         }
-      }
-      __syncthreads();
-      if (writer && row < rows) {
-        float4 v = *reinterpret_cast<const float4*>(merge + row * C::MERGE_LD + entry);
+    } else {
 #pragma unroll
-        for (int w = 1; w < PA_WARPS; ++w) {
-          const float4 u = *reinterpret_cast<const float4*>(merge + (w * C::ROWS + row) * C::MERGE_LD + entry);
-          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      for (int j = 0; j < RT; ++j) {
+        if (j * 8 >= rows) break;
+        float factor[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float sum = l[2 * j + c];
+          factor[c] = sum == 0.f ? 0.f : 1.f / sum;
+          if constexpr (C::E4M3) factor[c] *= a.v_scale[kv_head];
+          if (g == 0 && j * 8 + 2 * t4 + c < rows) paged_lse(a, r.s0, kv_head, row0 + j * 8 + 2 * t4 + c, m[2 * j + c], sum);
         }
-        const int d0 = merge_dim<C>(pass, entry), d1 = merge_dim<C>(pass, entry + 2);
-        if (partial) {
-          *reinterpret_cast<float2*>(out_part + d0) = make_float2(v.x, v.y);
-          *reinterpret_cast<float2*>(out_part + d1) = make_float2(v.z, v.w);
-        } else {
-          *reinterpret_cast<uint32_t*>(out + d0) = pack2<BF16>(v.x * factor, v.y * factor);
-          *reinterpret_cast<uint32_t*>(out + d1) = pack2<BF16>(v.z * factor, v.w * factor);
-        }
+        float f[C::DT][4];
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) f[dt][c] = o[dt][j][c];
+        store_frags<C, C::DT>(a, f, 0, factor, r.s0, kv_head, row0 + j * 8, rows - j * 8, lane);
       }
     }
-    __syncthreads();
 
     // ---- what the join needs to know
-    if (first_segment && !from_start) {  // the block that holds the unit's last tile
-      const long long end = t + (r.tiles - cur.tile);
+    if (first_segment && !from_start) {
+      const long long end = t + (r.steps - cur.step);  // the worker that holds the unit's last step
       int c = static_cast<int>(min((end * shares - 1) / total, static_cast<long long>(shares - 1)));
       while (c + 1 < shares && paged_border(total, shares, c + 1) < end) ++c;
       while (paged_border(total, shares, c) >= end) --c;
-      parts = c - block + 2;
+      mid0 = make_int4(c - worker + 2, 0, r.s0, kv_head);  // parts, from the worker before on
+      mid1 = make_int4(row0, rows, 0, 0);
     }
     if (from_start && !to_end) tail_slot = part;
     first_segment = false;
-    t += tiles;
+    t += steps;
     if (t < t1) cur.next_unit(a);
   }
-  if (tid == 0) *reinterpret_cast<int4*>(p.desc + block * PA_DESC) = make_int4(parts, z_first, sub_first, tail_slot);
+  if (lane == 0) {
+    mid0.y = tail_slot;
+    reinterpret_cast<int4*>(desc)[0] = mid0;
+    reinterpret_cast<int4*>(desc)[1] = mid1;
+  }
 }
 
-// Joins the parts of the units that borders between blocks cut.  The unit that block c comes in in the middle of
-// is listed for joining if block c - 1 began it.  Every block reads all descriptions, and rows of listed
-// units are dealt out: a unit of many parts (a long request has hundreds) takes a whole block a row, whose warps
-// share the parts; one of few takes a warp a row.
+// Joins the parts of the units that borders between workers cut.  The unit that worker c comes in in the middle of
+// is joined for c if worker c - 1 began it.  A warp takes a slice of the output's fragments of one such unit; a
+// unit of many parts (a long request has hundreds) takes the block, whose warps share the parts.
 constexpr int PA_JOIN_WARPS = 16;
-constexpr int PA_JOIN_MAX = 1024;  // blocks of the attention kernel
-constexpr int PA_JOIN_MANY = 16;   // parts from which on a row takes a block
+constexpr int PA_JOIN_MANY = 16;  // parts from which on a slice takes the block
 
 template <typename C>
-__device__ __forceinline__ void paged_join_store(const PagedAttnParams& p, const PagedRequest& r, int kv_head, int unit_row, int lane,
-                                                 const float2 (&v)[C::D / 64], float top, float sum) {
-  using T = typename C::type;
-  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  const syn_paged_attn_args& a = p.a;
-  const int group = a.Hq / a.Hkv;
-  float factor = sum == 0.f ? 0.f : 1.f / sum;
-  if constexpr (C::E4M3) factor *= a.v_scale[kv_head];
-  const int tok = unit_row / group, head = kv_head * group + unit_row - tok * group;
-  T* out = static_cast<T*>(a.o) + static_cast<int64_t>(r.s0 + tok) * a.o_strides[0] + head * a.o_strides[1];
+struct PagedJoinCfg {
+  static constexpr int SLICE = C::DT % 4 == 0 && C::FRAGS > 16 ? 4 : C::FRAGS > 8 ? 2 : 1;  // fragments a warp, of one row tile
+  static constexpr int SLICES = C::FRAGS / SLICE;
+};
+
+template <int N>
+struct PagedSum {
+  float m[2], l[2], o[N][4];
+  __device__ __forceinline__ void clear() {
+    m[0] = m[1] = -CUDART_INF_F, l[0] = l[1] = 0.f;
 #pragma unroll
-  for (int j = 0; j < C::D / 64; ++j)
-    *reinterpret_cast<uint32_t*>(out + j * 64 + lane * 2) = pack2<BF16>(v[j].x * factor, v[j].y * factor);
-  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(r.s0 + tok) * a.Hq + head] = top + log2f(sum);
-}
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+  }
+  __device__ __forceinline__ void add(const float4& ml, const float4 (&u)[N]) {
+    const float um[2] = {ml.x, ml.z}, ul[2] = {ml.y, ml.w};
+    float mine[2], other[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float top = fmaxf(m[c], um[c]), zero = top == -CUDART_INF_F ? 0.f : top;
+      mine[c] = ex2(m[c] - zero), other[c] = ex2(um[c] - zero);
+      m[c] = top;
+      l[c] = l[c] * mine[c] + ul[c] * other[c];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      o[i][0] = o[i][0] * mine[0] + u[i].x * other[0];
+      o[i][1] = o[i][1] * mine[1] + u[i].y * other[1];
+      o[i][2] = o[i][2] * mine[0] + u[i].z * other[0];
+      o[i][3] = o[i][3] * mine[1] + u[i].w * other[1];
+    }
+  }
+};
 
 template <typename C>
 __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-  constexpr int N = C::D / 64;  // pairs of columns a lane
-  __shared__ float2 s_o[PA_JOIN_WARPS][C::D / 2];
-  __shared__ float s_m[PA_JOIN_WARPS], s_l[PA_JOIN_WARPS];
-  __shared__ int16_t s_list[2][PA_JOIN_MAX];
-  __shared__ int s_found[2][PA_JOIN_WARPS];
+  constexpr int N = PagedJoinCfg<C>::SLICE, RT = C::RT;
+  __shared__ float4 s_ml[PA_JOIN_WARPS][32], s_o[PA_JOIN_WARPS][N][32];
+  __shared__ int s_many[PA_JOIN_WARPS];
   const syn_paged_attn_args& a = p.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int group = a.Hq / a.Hkv;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int c = 1 + blockIdx.x * PA_JOIN_WARPS + warp;
+  const int j = blockIdx.y % RT, dt = blockIdx.y / RT * N;  // row tile and first 16-dimension tile of the slice
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int count[2] = {0, 0};
-  for (int c0 = 1; c0 < p.grid; c0 += PA_JOIN_WARPS * 32) {  // in the order of the blocks: all have the same lists
-    const int c = c0 + threadIdx.x;
-    bool listed = false, many = false;
-    if (c < p.grid) {
-      const int parts = p.desc[c * PA_DESC];
-      listed = parts > 0 && p.desc[(c - 1) * PA_DESC + 3] >= 0;
-      many = parts >= PA_JOIN_MANY;
-    }
-    const unsigned mask[2] = {__ballot_sync(~0u, listed && many), __ballot_sync(~0u, listed && !many)};
-    __syncthreads();
-    if (lane < 2) s_found[lane][warp] = __popc(mask[lane]);
-    __syncthreads();
+
+  auto merge = [&](PagedSum<N>& sum, int c, int before, int parts, int from, int skip) {
+#pragma unroll 4
+    for (int i = from; i < parts; i += skip) {
+      const int64_t slot = i == 0 ? before : 2 * (c - 1 + i);
+      const float4 ml = *reinterpret_cast<const float4*>(p.part_ml + (slot * C::ROWS + j * 8 + 2 * t4) * 2);
+      float4 u[N];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      int at = count[k];
-      for (int w = 0; w < PA_JOIN_WARPS; ++w) {
-        if (w < warp) at += s_found[k][w];
-        count[k] += s_found[k][w];
+      for (int k = 0; k < N; ++k) u[k] = reinterpret_cast<const float4*>(p.part_o)[(slot * C::FRAGS + (dt + k) * RT + j) * 32 + lane];
+      sum.add(ml, u);
+    }
+  };
+  auto store = [&](const PagedSum<N>& sum, const int4& d0, const int4& d1) {
+    float factor[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      factor[x] = sum.l[x] == 0.f ? 0.f : 1.f / sum.l[x];
+      if constexpr (C::E4M3) factor[x] *= a.v_scale[d0.w];
+      const int row = j * 8 + 2 * t4 + x;
+      if (dt == 0 && g == 0 && row < d1.y) paged_lse(a, d0.z, d0.w, d1.x + row, sum.m[x], sum.l[x]);
+    }
+    store_frags<C, N>(a, sum.o, dt, factor, d0.z, d0.w, d1.x + j * 8, d1.y - j * 8, lane);
+  };
+
+  int parts = 0;
+  PagedSum<N> sum;
+  if (c < p.workers) {
+    const int4 d0 = reinterpret_cast<const int4*>(p.desc + c * PA_DESC)[0], d1 = reinterpret_cast<const int4*>(p.desc + c * PA_DESC)[1];
+    const int before = p.desc[(c - 1) * PA_DESC + 1];
+    if (d0.x > 0 && before >= 0 && j * 8 < d1.y) {
+      parts = d0.x;
+      if (parts < PA_JOIN_MANY) {
+        sum.clear();
+        const bool live = j * 8 + 2 * t4 < d1.y;  // lanes of rows that there are none of have nothing to read
+        merge(sum, c, before, live ? parts : 0, 0, 1);
+        store(sum, d0, d1);
       }
-      if (listed && many == (k == 0)) s_list[k][at + __popc(mask[k] & ((1u << lane) - 1))] = static_cast<int16_t>(c);
     }
   }
+  if (lane == 0) s_many[warp] = parts >= PA_JOIN_MANY;
   __syncthreads();
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    const int wide = k == 0 ? PA_JOIN_WARPS : 1;  // warps a row
-    const int share = k == 0 ? warp : 0;
-    const int items = count[k] * C::ROWS;
-    const int from = k == 0 ? blockIdx.x : blockIdx.x * PA_JOIN_WARPS + warp;
-    const int skip = k == 0 ? gridDim.x : gridDim.x * PA_JOIN_WARPS;
-    for (int item = from; item < items; item += skip) {
-      const int c = s_list[k][item / C::ROWS], row = item % C::ROWS;
-      const int4 d = *reinterpret_cast<const int4*>(p.desc + c * PA_DESC);
-      const int before = p.desc[(c - 1) * PA_DESC + 3], parts = d.x;
-      const PagedRequest r = paged_request<C>(a, d.y);
-      const int kv_head = d.z / r.rt, row0 = (d.z - kv_head * r.rt) * C::ROWS;
-      if (row >= r.n * group - row0) continue;
-      auto slot = [&](int i) { return i == 0 ? before : 2 * (c - 1 + i); };
-      float top = -CUDART_INF_F, sum = 0.f;
-      float2 v[N];
+  for (int w = 0; w < PA_JOIN_WARPS; ++w) {
+    if (!s_many[w]) continue;
+    const int cw = 1 + blockIdx.x * PA_JOIN_WARPS + w;
+    const int4 d0 = reinterpret_cast<const int4*>(p.desc + cw * PA_DESC)[0], d1 = reinterpret_cast<const int4*>(p.desc + cw * PA_DESC)[1];
+    const int before = p.desc[(cw - 1) * PA_DESC + 1];
+    const bool live = j * 8 + 2 * t4 < d1.y;
+    sum.clear();
+    merge(sum, cw, before, live ? d0.x : 0, warp, PA_JOIN_WARPS);
+    s_ml[warp][lane] = make_float4(sum.m[0], sum.l[0], sum.m[1], sum.l[1]);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
-      for (int i0 = share; i0 < parts; i0 += 32 * wide) {  // a part's statistics a lane, then one part after the other
-        const int i = i0 + lane * wide;
-        float2 ml = make_float2(-CUDART_INF_F, 0.f);
-        if (i < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + (static_cast<int64_t>(slot(i)) * C::ROWS + row) * 2);
-        float now = fmaxf(top, ml.x);
-        for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(~0u, now, d));
-        const float zero = now == -CUDART_INF_F ? 0.f : now, alpha = ex2(top - zero);
-        top = now;
-        const float w = ex2(ml.x - zero);
-        float more = ml.y * w;
-        for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(~0u, more, d);
-        sum = sum * alpha + more;
+    for (int k = 0; k < N; ++k) s_o[warp][k][lane] = make_float4(sum.o[k][0], sum.o[k][1], sum.o[k][2], sum.o[k][3]);
+    __syncthreads();
+    if (warp == 0) {
+      for (int v = 1; v < PA_JOIN_WARPS; ++v) {
+        float4 u[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j].x *= alpha, v[j].y *= alpha;
-        const int count = min(32, (parts - i0 + wide - 1) / wide);
-#pragma unroll 8
-        for (int q = 0; q < count; ++q) {
-          const float f = __shfl_sync(~0u, w, q);
-          const float* at = p.part_o + (static_cast<int64_t>(slot(i0 + q * wide)) * C::ROWS + row) * C::D + lane * 2;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float2 u = *reinterpret_cast<const float2*>(at + j * 64);
-            v[j].x += u.x * f, v[j].y += u.y * f;
-          }
-        }
+        for (int k = 0; k < N; ++k) u[k] = s_o[v][k][lane];
+        sum.add(s_ml[v][lane], u);
       }
-      if (k == 0) {
-        __syncthreads();
-        if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
-#pragma unroll
-        for (int j = 0; j < N; ++j) s_o[warp][j * 32 + lane] = v[j];
-        __syncthreads();
-        if (warp > 0) continue;
-        for (int w = 1; w < PA_JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
-        const float zero = top == -CUDART_INF_F ? 0.f : top;
-        sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = make_float2(0.f, 0.f);
-        for (int w = 0; w < PA_JOIN_WARPS; ++w) {
-          const float f = ex2(s_m[w] - zero);
-          sum += s_l[w] * f;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float2 u = s_o[w][j * 32 + lane];
-            v[j].x += u.x * f, v[j].y += u.y * f;
-          }
-        }
-      }
-      paged_join_store<C>(p, r, kv_head, row0 + row, lane, v, top, sum);
+      store(sum, d0, d1);
     }
+    __syncthreads();
   }
 }
 

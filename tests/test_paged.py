@@ -183,7 +183,8 @@ def test_c_entry_points_refuse_on_the_host():
                          (dict(num_pages=1 << 28), -9)]:
         assert lib.syn_paged_attention(_struct(L.PagedAttnArgs, **{**ok, **change}), None) == code, change
     assert lib.syn_paged_attention(_struct(L.PagedAttnArgs, **{**ok, "tokens": 0}), None) == 0
-    assert lib.syn_paged_attention_workspace(148) >= 0 and lib.syn_paged_attention_workspace(-1) < 0
+    assert lib.syn_paged_attention_workspace(148, 128) > 0
+    assert lib.syn_paged_attention_workspace(0, 128) == -1 and lib.syn_paged_attention_workspace(148, 96) == -8
     assert lib.syn_strerror(-10) != b"unknown error" and lib.syn_strerror(-11) != b"unknown error"
 
 
