@@ -48,9 +48,9 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
   if (rc != SYN_OK) return rc;
   PagedAttnParams p;
   p.a = a;
-  const int grid = sms * C::BLOCKS;
-  p.workers = grid * PA_WARPS;
-  p.min_steps = 4;
+  p.grid = sms * C::BLOCKS;
+  const int warps = p.grid * PA_WARPS;
+  p.min_steps = 2;
   // mulhi(n, 2^(31 + b) / d rounded up) >> (b - 1) = n / d for 0 <= n < 2^31, 2^(b - 1) < d <= 2^b
   p.page_mul = 0, p.page_shift = 0;
   if (a.page_size > 1) {
@@ -60,16 +60,17 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
     p.page_shift = b - 1;
   }
   p.desc = static_cast<int32_t*>(a.workspace);
-  p.part_ml = reinterpret_cast<float*>(p.desc + p.workers * PA_DESC);
-  p.part_o = p.part_ml + static_cast<int64_t>(2) * p.workers * C::ROWS * 2;
-  paged_attn_kernel<C><<<grid, PA_THREADS, C::SMEM, stream>>>(p);
+  p.part_ml = reinterpret_cast<float*>(p.desc + warps * PA_DESC);
+  p.part_o = p.part_ml + static_cast<int64_t>(2) * warps * C::ROWS * 2;
+  paged_attn_kernel<C><<<p.grid, PA_THREADS, C::SMEM, stream>>>(p);
   SYN_CUDA_TRY(cudaGetLastError());
   // The join's blocks are brought in while the last shares are still at work and wait for them there.
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((p.workers - 2) / PA_JOIN_WARPS + 1, PagedJoinCfg<C>::SLICES);
+  const PagedJoinGrid<C> join(warps);
+  config.gridDim = dim3(join.few + join.many);
   config.blockDim = dim3(PA_JOIN_WARPS * 32);
   config.stream = stream;
   config.attrs = &attr;

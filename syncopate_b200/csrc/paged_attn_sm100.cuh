@@ -11,11 +11,12 @@
 // dimensions by rows) because rows then come in eights, as groups do, and not in sixteens.  The layout is chosen
 // for loads in flight:
 //   * Every warp is a worker of its own: it streams its keys and values through a ring of its own in shared memory
-//     (cp.async of 16 bytes, a page lookup a step), with no barrier between the warps of a block.
+//     (cp.async of 16 bytes, a page lookup a step), with no barrier between the warps of a block on the way.
 //   * The work (requests x key-value heads x row tiles x steps of keys) is laid out in one line and cut into
 //     equal shares for the warps of a grid that fills the GPU, whatever the lengths; loads run on across the
 //     borders of units.  A unit that a border cuts leaves partial results, which a second small kernel joins
-//     in a fixed order: results do not depend on timing, there are no atomics and no state between calls.
+//     in a fixed order (the warps of a block that work on one and the same unit join theirs first): results do
+//     not depend on timing, there are no atomics and no state between calls.
 #pragma once
 #include <math_constants.h>
 
@@ -30,18 +31,35 @@ constexpr int PA_THREADS = PA_WARPS * 32;
 // The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
 // than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
 constexpr float PA_SLACK = 8.f;
-constexpr int PA_DESC = 8;  // int32 words a worker leaves for the join
+constexpr int PA_DESC = 12;  // int32 words a worker leaves for the join (PagedJoin)
 
 struct PagedAttnParams {
   syn_paged_attn_args a;
-  int32_t workers;    // warps of the launch
+  int32_t grid;       // blocks of the launch
   int32_t min_steps;  // fewest steps worth a worker
   uint32_t page_mul;  // key / page_size = mulhi(key, page_mul) >> page_shift (page_mul 0: pages of one key)
   int32_t page_shift;
-  float* part_o;      // [2 * workers][fragments of the output: D / 16, 8-row tiles][lanes][4]
-  float* part_ml;     // [2 * workers][rows of a unit][2]
-  int32_t* desc;      // [workers][PA_DESC]
+  float* part_o;      // [2 * warps][fragments of the output: D / 16, 8-row tiles][lanes][4]
+  float* part_ml;     // [2 * warps][rows of a unit][2]
+  int32_t* desc;      // [warps][PA_DESC]
 };
+
+// A unit that borders cut, as left by the second worker on it.  Its parts in order: `n1` of single workers (the
+// first in slot `slot1`, then slot 2 w of the workers that follow worker w1), `n2` of blocks (slot 2 wide b of
+// block b2 and those that follow), `n3` of single workers (from w3 on).
+struct alignas(16) PagedJoin {
+  int n1, slot1, w1;
+  int n2, b2, wide;
+  int n3, w3;
+  int s0, kv_head, row0, rows;
+  __device__ __forceinline__ int parts() const { return n1 + n2 + n3; }
+  __device__ __forceinline__ int slot(int i) const {
+    if (i < n1) return i == 0 ? slot1 : 2 * (w1 + i);
+    i -= n1;
+    return i < n2 ? 2 * wide * (b2 + i) : 2 * (w3 + i - n2);
+  }
+};
+static_assert(sizeof(PagedJoin) == PA_DESC * 4, "PagedJoin");
 
 template <typename T, bool E4M3_, int D_, int RT_>
 struct PagedCfg {
@@ -64,6 +82,7 @@ struct PagedCfg {
   static constexpr int QB = QREG ? 0 : KSTEPS * RT * 256;
   static constexpr int SMEM = PA_WARPS * (RING + QB);
   static_assert(BLOCKS * (SMEM + 1280) <= 228 * 1024, "shared memory of an SM");
+  static_assert(RING >= FRAGS * 512 + RT * 512, "the parts of a pooled block");
   static_assert(SLOTS >= 3, "a key half, a value half and one on its way");
 };
 
@@ -174,7 +193,23 @@ __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args&
   return r;
 }
 
-__device__ __forceinline__ long long paged_border(long long total, int shares, int c) { return total * c / shares; }
+// The line cut into `shares` pieces: the first `more` of them have one step more than the others.
+struct PagedCut {
+  long long each;
+  int shares, more;
+  __device__ __forceinline__ PagedCut(long long total, int shares_) : shares(shares_) {
+    each = total <= UINT_MAX ? static_cast<uint32_t>(total) / static_cast<uint32_t>(shares) : total / shares;
+    more = static_cast<int>(total - each * shares);
+  }
+  __device__ __forceinline__ long long at(int c) const { return c * each + min(c, more); }  // where piece c begins
+  __device__ __forceinline__ int piece(long long step) const {  // the piece that a step lies in
+    const long long longer = more * (each + 1);
+    return step < longer ? quotient(step, each + 1) : more + quotient(step - longer, each);
+  }
+  static __device__ __forceinline__ int quotient(long long n, long long d) {
+    return static_cast<int>(n <= UINT_MAX ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d);
+  }
+};
 
 // Position on the line: step `step` of unit `sub` (head * row tiles + row tile) of request z.
 template <typename C>
@@ -320,6 +355,52 @@ __device__ __forceinline__ void store_frags(const syn_paged_attn_args& a, const 
   }
 }
 
+// Rows of COUNT output fragments whose sums are complete: divided, stored, and their log-sum-exp with the first.
+template <typename C, int COUNT>
+__device__ __forceinline__ void paged_finish(const syn_paged_attn_args& a, const float (&o)[COUNT][4], const float (&m)[2],
+                                             const float (&l)[2], int dt, int s0, int kv_head, int unit_row, int rows, int lane) {
+  float factor[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int row = 2 * (lane & 3) + c;
+    factor[c] = l[c] == 0.f ? 0.f : 1.f / l[c];
+    if constexpr (C::E4M3) factor[c] *= a.v_scale[kv_head];
+    if (dt == 0 && lane < 4 && row < rows) paged_lse(a, s0, kv_head, unit_row + row, m[c], l[c]);
+  }
+  store_frags<C, COUNT>(a, o, dt, factor, s0, kv_head, unit_row, rows, lane);
+}
+
+// Output fragments of parts of a unit's keys, joined one after the other.
+template <int N>
+struct PagedSum {
+  float m[2], l[2], o[N][4];
+  __device__ __forceinline__ void clear() {
+    m[0] = m[1] = -CUDART_INF_F, l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+  }
+  __device__ __forceinline__ void add(const float4& ml, const float4 (&u)[N]) {
+    const float um[2] = {ml.x, ml.z}, ul[2] = {ml.y, ml.w};
+    float mine[2], other[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float top = fmaxf(m[c], um[c]), zero = top == -CUDART_INF_F ? 0.f : top;
+      mine[c] = ex2(m[c] - zero), other[c] = ex2(um[c] - zero);
+      m[c] = top;
+      l[c] = l[c] * mine[c] + ul[c] * other[c];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      o[i][0] = o[i][0] * mine[0] + u[i].x * other[0];
+      o[i][1] = o[i][1] * mine[1] + u[i].y * other[1];
+      o[i][2] = o[i][2] * mine[0] + u[i].z * other[0];
+      o[i][3] = o[i][3] * mine[1] + u[i].w * other[1];
+    }
+  }
+};
+
 template <typename C>
 __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
   using T = typename C::type;
@@ -359,11 +440,13 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     if (w < warp) upto += s_sum[w];
     total += s_sum[w];
   }
-  const int shares = static_cast<int>(min(static_cast<long long>(p.workers), max(1LL, total / p.min_steps)));
+  const int shares = static_cast<int>(min(static_cast<long long>(p.grid) * PA_WARPS, max(1LL, total / p.min_steps)));
+  constexpr int wide = PA_WARPS;
+  const PagedCut cut(total, shares);
 #pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) {  // neighbouring shares go to different blocks
-    const int share = w * gridDim.x + blockIdx.x;
-    const long long from = share < shares ? paged_border(total, shares, share) : total;
+  for (int w = 0; w < PA_WARPS; ++w) {
+    const int share = blockIdx.x * wide + w;
+    const long long from = w < wide && share < shares ? cut.at(share) : total;
     if (upto - mine <= from && from < upto) {
       long long rest = from - (upto - mine);
       int z = z0;
@@ -377,18 +460,52 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       s_rest[w] = rest;
     }
   }
-  __syncthreads();  // the last barrier: from here on the warps go their own ways
-  const int worker = warp * gridDim.x + blockIdx.x;
-  int32_t* desc = p.desc + worker * PA_DESC;
-  const long long t0 = worker < shares ? paged_border(total, shares, worker) : total;
-  const long long t1 = worker < shares ? paged_border(total, shares, worker + 1) : total;
+  __syncthreads();  // from here on the warps go their own ways
+  // Every warp has a record: those without work one of nothing to join.
+  int32_t* const record = p.desc + (blockIdx.x * PA_WARPS + warp) * PA_DESC;
+  const int worker = blockIdx.x * wide + warp;
+  const bool works = warp < wide && worker < shares;
+  const long long t0 = works ? cut.at(worker) : total;
+  const long long t1 = works ? cut.at(worker + 1) : total;
+  PagedJoin join;
+  join.n1 = join.n2 = join.n3 = 0;
   if (t0 >= t1) {
-    if (lane == 0) *reinterpret_cast<int4*>(desc) = make_int4(0, -1, 0, 0);
+    if (lane == 0) *reinterpret_cast<int4*>(record) = make_int4(0, 0, 0, 0), reinterpret_cast<int4*>(record)[1] = make_int4(0, 0, 0, 0);
     return;
   }
 
   PagedCursor<C> cur;
   cur.at(a, s_z[warp], s_rest[warp]);
+  const long long unit0 = t0 - cur.step, unit1 = unit0 + cur.r.steps;  // the first unit, on the line
+  // A block all of whose shares lie in one unit joins its warps' parts itself.
+  auto pooled = [&](int block) {
+    return wide > 1 && cut.at(block * wide) >= unit0 &&
+           cut.at(min((block + 1) * wide, shares)) <= unit1;
+  };
+  const bool pool = pooled(blockIdx.x);
+  if (worker > 0 && cur.step > 0 && cut.at(worker - 1) <= unit0) {  // the second worker on the unit
+    const int first = worker - 1, b_first = first / wide;
+    const int last = cut.piece(unit1 - 1), b_last = last / wide;
+    const bool pool_first = pooled(b_first), pool_last = pooled(b_last);
+    join.slot1 = 2 * first + (cut.at(first) != unit0), join.w1 = first;
+    join.wide = wide, join.w3 = b_last * wide;
+    if (b_first == b_last) {
+      join.n1 = pool_first ? 0 : last - first + 1;  // pooled: the block has the whole unit
+      join.b2 = 0;
+    } else {
+      join.n1 = pool_first ? 0 : (b_first + 1) * wide - first;
+      join.b2 = pool_first ? b_first : b_first + 1;
+      join.n2 = (pool_last ? b_last + 1 : b_last) - join.b2;
+      join.n3 = pool_last ? 0 : last - join.w3 + 1;
+    }
+    const int head = cur.sub / cur.r.rt;
+    join.s0 = cur.r.s0, join.kv_head = head, join.row0 = (cur.sub - head * cur.r.rt) * C::ROWS;
+    join.rows = min(C::ROWS, cur.r.n * group - join.row0);
+  }
+  if (lane == 0) {
+    if (join.parts() > 0) *reinterpret_cast<PagedJoin*>(record) = join;
+    else *reinterpret_cast<int4*>(record) = make_int4(0, 0, 0, 0), reinterpret_cast<int4*>(record)[1] = make_int4(0, 0, 0, 0);
+  }
 
   // ---- producer: halves of steps (keys, values, keys, ...) are asked for SLOTS - 1 halves ahead, across units
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
@@ -476,8 +593,6 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
   const uint32_t q_smem = smem_u32(smem) + PA_WARPS * C::RING + warp * C::QB;
   long long t = t0;
-  int tail_slot = -1;  // part of the unit that this worker begins and does not end
-  int4 mid0 = make_int4(0, 0, 0, 0), mid1 = mid0;  // the unit that it comes in in the middle of
   bool first_segment = true;
 
   while (t < t1) {
@@ -486,6 +601,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const int kv_head = cur.sub / r.rt, row0 = (cur.sub - kv_head * r.rt) * C::ROWS;
     const int rows = min(C::ROWS, r.n * group - row0);
     const int pos0 = r.len - r.n;
+    const bool one = r.n == 1;  // one new token: spares the divisions
     const int steps = static_cast<int>(min(static_cast<long long>(r.steps - cur.step), t1 - t));
     // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
     // Rows behind the last repeat it.
@@ -493,7 +609,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     float mult[2 * RT];
 #pragma unroll
     for (int x = 0; x < 2 * RT; ++x) {
-      const int tok = (row0 + min((x >> 1) * 8 + 2 * t4 + (x & 1), rows - 1)) / group;
+      const int tok = one ? 0 : (row0 + min((x >> 1) * 8 + 2 * t4 + (x & 1), rows - 1)) / group;
       hi[x] = a.causal ? min(r.len, pos0 + tok + 1) : r.len;
       lo[x] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
       mult[x] = a.sm_scale * CUDART_L2E_F;
@@ -502,10 +618,10 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const T* qrow[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const int row = row0 + min(8 * i + g, rows - 1), tok = row / group, head = kv_head * group + row - tok * group;
+      const int row = row0 + min(8 * i + g, rows - 1), tok = one ? 0 : row / group, head = kv_head * group + row - tok * group;
       qrow[i] = static_cast<const T*>(a.q) + static_cast<int64_t>(r.s0 + tok) * a.q_strides[0] + head * a.q_strides[1];
     }
-    const int tok_a = row0 / group, tok_b = (row0 + rows - 1) / group;
+    const int tok_a = one ? 0 : row0 / group, tok_b = one ? 0 : (row0 + rows - 1) / group;
     const int all_lo = a.window > 0 ? max(0, pos0 + tok_b - a.window + 1) : 0;  // keys that every row sees
     const int all_hi = a.causal ? min(r.len, pos0 + tok_a + 1) : r.len;
 
@@ -785,6 +901,45 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       l[x] += __shfl_xor_sync(~0u, l[x], 16);
       if (slack[x] == -CUDART_INF_F) m[x] = -CUDART_INF_F;
     }
+    if (pool) {
+      // The warps' parts meet in shared memory, in place of the rings, and each warp joins some fragments.
+      cp_async_wait<0>();
+      __syncwarp();
+      const int active = min(wide, shares - static_cast<int>(blockIdx.x) * wide);
+      auto own_o = [&](int w) { return reinterpret_cast<float4*>(smem + w * C::RING) + lane; };
+      auto own_ml = [&](int w) { return reinterpret_cast<float4*>(smem + w * C::RING + C::FRAGS * 512) + lane; };
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+          own_o(warp)[(dt * RT + j) * 32] = make_float4(o[dt][j][0], o[dt][j][1], o[dt][j][2], o[dt][j][3]);
+        own_ml(warp)[j * 32] = make_float4(m[2 * j], l[2 * j], m[2 * j + 1], l[2 * j + 1]);
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(active * 32) : "memory");
+      const bool all = unit0 == cut.at(blockIdx.x * wide) &&
+                       unit1 == cut.at(min((static_cast<int>(blockIdx.x) + 1) * wide, shares));
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) * wide;
+#pragma unroll 1
+      for (int f = warp; f < C::FRAGS; f += active) {
+        const int dt = f / RT, j = f % RT;
+        PagedSum<1> sum;
+        sum.clear();
+#pragma unroll 1
+        for (int w = 0; w < active; ++w) {
+          const float4 u[1] = {own_o(w)[f * 32]};
+          sum.add(own_ml(w)[j * 32], u);
+        }
+        if (j * 8 >= rows) continue;
+        if (all) {
+          paged_finish<C, 1>(a, sum.o, sum.m, sum.l, dt, r.s0, kv_head, row0 + j * 8, rows - j * 8, lane);
+        } else if (j * 8 + 2 * t4 < rows) {
+          reinterpret_cast<float4*>(p.part_o)[(slot * C::FRAGS + f) * 32 + lane] = make_float4(sum.o[0][0], sum.o[0][1], sum.o[0][2], sum.o[0][3]);
+          if (dt == 0 && g == 0)
+            *reinterpret_cast<float4*>(p.part_ml + (slot * C::ROWS + j * 8 + 2 * t4) * 2) = make_float4(sum.m[0], sum.l[0], sum.m[1], sum.l[1]);
+        }
+      }
+      return;
+    }
     if (partial) {
       float4* to = reinterpret_cast<float4*>(p.part_o) + static_cast<int64_t>(part) * C::FRAGS * 32 + lane;
 #pragma unroll
@@ -801,157 +956,110 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
         if (j * 8 >= rows) break;
-        float factor[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float sum = l[2 * j + c];
-          factor[c] = sum == 0.f ? 0.f : 1.f / sum;
-          if constexpr (C::E4M3) factor[c] *= a.v_scale[kv_head];
-          if (g == 0 && j * 8 + 2 * t4 + c < rows) paged_lse(a, r.s0, kv_head, row0 + j * 8 + 2 * t4 + c, m[2 * j + c], sum);
-        }
         float f[C::DT][4];
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) f[dt][c] = o[dt][j][c];
-        store_frags<C, C::DT>(a, f, 0, factor, r.s0, kv_head, row0 + j * 8, rows - j * 8, lane);
+        const float sum[2] = {l[2 * j], l[2 * j + 1]}, ref[2] = {m[2 * j], m[2 * j + 1]};
+        paged_finish<C, C::DT>(a, f, ref, sum, 0, r.s0, kv_head, row0 + j * 8, rows - j * 8, lane);
       }
     }
-
-    // ---- what the join needs to know
-    if (first_segment && !from_start) {
-      const long long end = t + (r.steps - cur.step);  // the worker that holds the unit's last step
-      int c = static_cast<int>(min((end * shares - 1) / total, static_cast<long long>(shares - 1)));
-      while (c + 1 < shares && paged_border(total, shares, c + 1) < end) ++c;
-      while (paged_border(total, shares, c) >= end) --c;
-      mid0 = make_int4(c - worker + 2, 0, r.s0, kv_head);  // parts, from the worker before on
-      mid1 = make_int4(row0, rows, 0, 0);
-    }
-    if (from_start && !to_end) tail_slot = part;
     first_segment = false;
     t += steps;
     if (t < t1) cur.next_unit(a);
   }
-  if (lane == 0) {
-    mid0.y = tail_slot;
-    reinterpret_cast<int4*>(desc)[0] = mid0;
-    reinterpret_cast<int4*>(desc)[1] = mid1;
+}
+
+// Joins the parts of the units that borders between workers cut.  Of a unit of few parts a warp takes four fragments
+// of the output; of one of many (a long request has hundreds) a block takes a fragment, and its warps share the
+// parts.  The kernel runs for a few microseconds, most of which its first pass through its own code takes: the
+// loops stay rolled up (unrolled by 4 over parts and by 8 over fragments it took 24 us on 1776 units of two parts).
+constexpr int PA_JOIN_WARPS = 16;
+constexpr int PA_JOIN_MANY = 12;    // parts from which on a unit counts as one of many
+constexpr int PA_JOIN_FRAGS = 4;    // fragments a warp, of one 8-row tile
+constexpr int PA_JOIN_LOOK = 128;   // records that a block looks through for units of many parts
+
+// Blocks of the join: those for units of few parts, then those for units of many.
+template <typename C>
+struct PagedJoinGrid {
+  static constexpr int SLICES = C::FRAGS / PA_JOIN_FRAGS;
+  int few, many;
+  __host__ __device__ explicit PagedJoinGrid(int records)
+      : few((records + PA_JOIN_WARPS - 1) / PA_JOIN_WARPS * SLICES), many((records + PA_JOIN_LOOK - 1) / PA_JOIN_LOOK * C::FRAGS) {}
+};
+
+// Adds parts from, from + skip, ... of N fragments, U of them on their way at a time.
+template <typename C, int N, int U>
+__device__ __forceinline__ void paged_merge(const PagedAttnParams& p, const PagedJoin& d, PagedSum<N>& sum, int dt, int j, int from,
+                                            int skip, int lane) {
+  const int t4 = lane & 3, parts = j * 8 + 2 * t4 < d.rows ? d.parts() : 0;  // rows that there are none of have nothing to read
+#pragma unroll 1
+  for (int i = from; i < parts; i += U * skip) {
+    float4 ml[U], u[U][N];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int64_t slot = d.slot(min(i + q * skip, parts - 1));
+      ml[q] = *reinterpret_cast<const float4*>(p.part_ml + (slot * C::ROWS + j * 8 + 2 * t4) * 2);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        u[q][k] = reinterpret_cast<const float4*>(p.part_o)[(slot * C::FRAGS + (dt + k) * C::RT + j) * 32 + lane];
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+      if (i + q * skip < parts) sum.add(ml[q], u[q]);
   }
 }
 
-// Joins the parts of the units that borders between workers cut.  The unit that worker c comes in in the middle of
-// is joined for c if worker c - 1 began it.  A warp takes a slice of the output's fragments of one such unit; a
-// unit of many parts (a long request has hundreds) takes the block, whose warps share the parts.
-constexpr int PA_JOIN_WARPS = 16;
-constexpr int PA_JOIN_MANY = 16;  // parts from which on a slice takes the block
-
-template <typename C>
-struct PagedJoinCfg {
-  static constexpr int SLICE = C::DT % 4 == 0 && C::FRAGS > 16 ? 4 : C::FRAGS > 8 ? 2 : 1;  // fragments a warp, of one row tile
-  static constexpr int SLICES = C::FRAGS / SLICE;
-};
-
-template <int N>
-struct PagedSum {
-  float m[2], l[2], o[N][4];
-  __device__ __forceinline__ void clear() {
-    m[0] = m[1] = -CUDART_INF_F, l[0] = l[1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-  }
-  __device__ __forceinline__ void add(const float4& ml, const float4 (&u)[N]) {
-    const float um[2] = {ml.x, ml.z}, ul[2] = {ml.y, ml.w};
-    float mine[2], other[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float top = fmaxf(m[c], um[c]), zero = top == -CUDART_INF_F ? 0.f : top;
-      mine[c] = ex2(m[c] - zero), other[c] = ex2(um[c] - zero);
-      m[c] = top;
-      l[c] = l[c] * mine[c] + ul[c] * other[c];
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      o[i][0] = o[i][0] * mine[0] + u[i].x * other[0];
-      o[i][1] = o[i][1] * mine[1] + u[i].y * other[1];
-      o[i][2] = o[i][2] * mine[0] + u[i].z * other[0];
-      o[i][3] = o[i][3] * mine[1] + u[i].w * other[1];
-    }
-  }
-};
-
 template <typename C>
 __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-  constexpr int N = PagedJoinCfg<C>::SLICE, RT = C::RT;
-  __shared__ float4 s_ml[PA_JOIN_WARPS][32], s_o[PA_JOIN_WARPS][N][32];
-  __shared__ int s_many[PA_JOIN_WARPS];
-  const syn_paged_attn_args& a = p.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  const int c = 1 + blockIdx.x * PA_JOIN_WARPS + warp;
-  const int j = blockIdx.y % RT, dt = blockIdx.y / RT * N;  // row tile and first 16-dimension tile of the slice
+  constexpr int RT = C::RT;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, records = p.grid * PA_WARPS;
+  const PagedJoinGrid<C> grid(records);
+  const PagedJoin* record = reinterpret_cast<const PagedJoin*>(p.desc);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  auto merge = [&](PagedSum<N>& sum, int c, int before, int parts, int from, int skip) {
-#pragma unroll 4
-    for (int i = from; i < parts; i += skip) {
-      const int64_t slot = i == 0 ? before : 2 * (c - 1 + i);
-      const float4 ml = *reinterpret_cast<const float4*>(p.part_ml + (slot * C::ROWS + j * 8 + 2 * t4) * 2);
-      float4 u[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) u[k] = reinterpret_cast<const float4*>(p.part_o)[(slot * C::FRAGS + (dt + k) * RT + j) * 32 + lane];
-      sum.add(ml, u);
-    }
-  };
-  auto store = [&](const PagedSum<N>& sum, const int4& d0, const int4& d1) {
-    float factor[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      factor[x] = sum.l[x] == 0.f ? 0.f : 1.f / sum.l[x];
-      if constexpr (C::E4M3) factor[x] *= a.v_scale[d0.w];
-      const int row = j * 8 + 2 * t4 + x;
-      if (dt == 0 && g == 0 && row < d1.y) paged_lse(a, d0.z, d0.w, d1.x + row, sum.m[x], sum.l[x]);
-    }
-    store_frags<C, N>(a, sum.o, dt, factor, d0.z, d0.w, d1.x + j * 8, d1.y - j * 8, lane);
-  };
-
-  int parts = 0;
-  PagedSum<N> sum;
-  if (c < p.workers) {
-    const int4 d0 = reinterpret_cast<const int4*>(p.desc + c * PA_DESC)[0], d1 = reinterpret_cast<const int4*>(p.desc + c * PA_DESC)[1];
-    const int before = p.desc[(c - 1) * PA_DESC + 1];
-    if (d0.x > 0 && before >= 0 && j * 8 < d1.y) {
-      parts = d0.x;
-      if (parts < PA_JOIN_MANY) {
-        sum.clear();
-        const bool live = j * 8 + 2 * t4 < d1.y;  // lanes of rows that there are none of have nothing to read
-        merge(sum, c, before, live ? parts : 0, 0, 1);
-        store(sum, d0, d1);
-      }
-    }
-  }
-  if (lane == 0) s_many[warp] = parts >= PA_JOIN_MANY;
-  __syncthreads();
-  for (int w = 0; w < PA_JOIN_WARPS; ++w) {
-    if (!s_many[w]) continue;
-    const int cw = 1 + blockIdx.x * PA_JOIN_WARPS + w;
-    const int4 d0 = reinterpret_cast<const int4*>(p.desc + cw * PA_DESC)[0], d1 = reinterpret_cast<const int4*>(p.desc + cw * PA_DESC)[1];
-    const int before = p.desc[(cw - 1) * PA_DESC + 1];
-    const bool live = j * 8 + 2 * t4 < d1.y;
+  if (static_cast<int>(blockIdx.x) < grid.few) {
+    const int slice = blockIdx.x % PagedJoinGrid<C>::SLICES, c = blockIdx.x / PagedJoinGrid<C>::SLICES * PA_JOIN_WARPS + warp;
+    const int j = slice % RT, dt = slice / RT * PA_JOIN_FRAGS;
+    if (c >= records) return;
+    const PagedJoin d = record[c];
+    if (d.parts() == 0 || d.parts() >= PA_JOIN_MANY || j * 8 >= d.rows) return;
+    PagedSum<PA_JOIN_FRAGS> sum;
     sum.clear();
-    merge(sum, cw, before, live ? d0.x : 0, warp, PA_JOIN_WARPS);
+    paged_merge<C, PA_JOIN_FRAGS, 2>(p, d, sum, dt, j, 0, 1, lane);
+    paged_finish<C, PA_JOIN_FRAGS>(p.a, sum.o, sum.m, sum.l, dt, d.s0, d.kv_head, d.row0 + j * 8, d.rows - j * 8, lane);
+    return;
+  }
+  __shared__ float4 s_ml[PA_JOIN_WARPS][32], s_o[PA_JOIN_WARPS][32];
+  __shared__ uint32_t s_many[PA_JOIN_LOOK / 32];
+  const int index = blockIdx.x - grid.few, f = index % C::FRAGS, c0 = index / C::FRAGS * PA_JOIN_LOOK;
+  const int j = f % RT, dt = f / RT;
+  int parts = 0;
+  if (threadIdx.x < PA_JOIN_LOOK && c0 + static_cast<int>(threadIdx.x) < records) parts = record[c0 + threadIdx.x].parts();
+  const uint32_t many = __ballot_sync(~0u, parts >= PA_JOIN_MANY);
+  if (lane == 0 && warp < PA_JOIN_LOOK / 32) s_many[warp] = many;
+  if (!__syncthreads_or(parts >= PA_JOIN_MANY)) return;
+  uint32_t left = s_many[0];
+#pragma unroll 1
+  for (int group = 0;;) {
+    while (left == 0 && ++group < PA_JOIN_LOOK / 32) left = s_many[group];
+    if (left == 0) return;
+    const PagedJoin d = record[c0 + group * 32 + __ffs(left) - 1];
+    left &= left - 1;
+    if (j * 8 >= d.rows) continue;
+    PagedSum<1> sum;
+    sum.clear();
+    paged_merge<C, 1, 4>(p, d, sum, dt, j, warp, PA_JOIN_WARPS, lane);
     s_ml[warp][lane] = make_float4(sum.m[0], sum.l[0], sum.m[1], sum.l[1]);
-#pragma unroll
-    for (int k = 0; k < N; ++k) s_o[warp][k][lane] = make_float4(sum.o[k][0], sum.o[k][1], sum.o[k][2], sum.o[k][3]);
+    s_o[warp][lane] = make_float4(sum.o[0][0], sum.o[0][1], sum.o[0][2], sum.o[0][3]);
     __syncthreads();
     if (warp == 0) {
+#pragma unroll 1
       for (int v = 1; v < PA_JOIN_WARPS; ++v) {
-        float4 u[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) u[k] = s_o[v][k][lane];
+        const float4 u[1] = {s_o[v][lane]};
         sum.add(s_ml[v][lane], u);
       }
-      store(sum, d0, d1);
+      paged_finish<C, 1>(p.a, sum.o, sum.m, sum.l, dt, d.s0, d.kv_head, d.row0 + j * 8, d.rows - j * 8, lane);
     }
     __syncthreads();
   }
