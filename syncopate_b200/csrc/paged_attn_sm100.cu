@@ -51,6 +51,9 @@ static int launch_paged(const syn_paged_attn_args& a, int sms, cudaStream_t stre
   p.grid = sms * C::BLOCKS;
   const int warps = p.grid * PA_WARPS;
   p.min_steps = 2;
+  p.tracks = 1;
+  if (a.cache_strides[2] * (C::E4M3 ? 1 : 2) == C::ROWB)
+    while (p.tracks * C::ROWB < 256 && a.Hkv % (2 * p.tracks) == 0) p.tracks *= 2;
   // mulhi(n, 2^(31 + b) / d rounded up) >> (b - 1) = n / d for 0 <= n < 2^31, 2^(b - 1) < d <= 2^b
   p.page_mul = 0, p.page_shift = 0;
   if (a.page_size > 1) {

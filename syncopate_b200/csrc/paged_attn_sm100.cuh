@@ -14,7 +14,9 @@
 //     (cp.async of 16 bytes, a page lookup a step), with no barrier between the warps of a block on the way.
 //   * The work (requests x key-value heads x row tiles x steps of keys) is laid out in one line and cut into
 //     equal shares for the warps of a grid that fills the GPU, whatever the lengths; loads run on across the
-//     borders of units.  A unit that a border cuts leaves partial results, which a second small kernel joins
+//     borders of units.  Where a head is less than 256 bytes and the heads of a token lie side by side, two or
+//     four warps take neighbouring heads at the same keys (`tracks`): HBM answers 128 bytes here and there a
+//     sixth slower than 256.  A unit that a border cuts leaves partial results, which a second small kernel joins
 //     in a fixed order (the warps of a block that work on one and the same unit join theirs first): results do
 //     not depend on timing, there are no atomics and no state between calls.
 #pragma once
@@ -31,12 +33,14 @@ constexpr int PA_THREADS = PA_WARPS * 32;
 // The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
 // than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
 constexpr float PA_SLACK = 8.f;
+constexpr float PA_NONE = -1e30f;
 constexpr int PA_DESC = 12;  // int32 words a worker leaves for the join (PagedJoin)
 
 struct PagedAttnParams {
   syn_paged_attn_args a;
   int32_t grid;       // blocks of the launch
   int32_t min_steps;  // fewest steps worth a worker
+  int32_t tracks;     // neighbouring heads that as many warps of a block take at the same keys (1, 2 or 4)
   uint32_t page_mul;  // key / page_size = mulhi(key, page_mul) >> page_shift (page_mul 0: pages of one key)
   int32_t page_shift;
   float* part_o;      // [2 * warps][fragments of the output: D / 16, 8-row tiles][lanes][4]
@@ -46,7 +50,8 @@ struct PagedAttnParams {
 
 // A unit that borders cut, as left by the second worker on it.  Its parts in order: `n1` of single workers (the
 // first in slot `slot1`, then slot 2 w of the workers that follow worker w1), `n2` of blocks (slot 2 wide b of
-// block b2 and those that follow), `n3` of single workers (from w3 on).
+// block b2 and those that follow), `n3` of single workers (from w3 on); `wide` workers a block.  With tracks
+// those are slots of a track.
 struct alignas(16) PagedJoin {
   int n1, slot1, w1;
   int n2, b2, wide;
@@ -54,9 +59,12 @@ struct alignas(16) PagedJoin {
   int s0, kv_head, row0, rows;
   __device__ __forceinline__ int parts() const { return n1 + n2 + n3; }
   __device__ __forceinline__ int slot(int i) const {
-    if (i < n1) return i == 0 ? slot1 : 2 * (w1 + i);
-    i -= n1;
-    return i < n2 ? 2 * wide * (b2 + i) : 2 * (w3 + i - n2);
+    int at;
+    if (i < n1) at = i == 0 ? slot1 : 2 * (w1 + i);
+    else if (i < n1 + n2) at = 2 * wide * (b2 + i - n1);
+    else at = 2 * (w3 + i - n1 - n2);
+    const int tracks = PA_WARPS / wide;
+    return at * tracks + kv_head % tracks;
   }
 };
 static_assert(sizeof(PagedJoin) == PA_DESC * 4, "PagedJoin");
@@ -72,8 +80,8 @@ struct PagedCfg {
   static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
   static constexpr int HALFB = KEYS * ROWB;          // the keys of a step, or its values
-  static constexpr int BLOCKS = D == 256 ? 3 - RT : RT <= 2 ? 3 : 2;  // resident on an SM
-  static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? (RT <= 2 ? 4 : 5) : (RT <= 2 ? 8 : 10);
+  static constexpr int BLOCKS = D == 256 ? 3 - RT : RT == 1 || (RT == 2 && D == 64) ? 3 : 2;  // resident on an SM
+  static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? (RT == 1 ? 4 : 5) : (RT <= 2 ? 8 : 10);
   static constexpr int RING = SLOTS * HALFB;         // bytes a warp
   static constexpr bool QREG = RT * D <= 256;        // query fragments in registers, else in shared memory
   static constexpr int KSTEPS = D / 16;
@@ -224,9 +232,9 @@ struct PagedCursor {
     step = static_cast<int>(rest % r.steps);
   }
   // To the first step of the next unit; the caller knows that there is one.
-  __device__ __forceinline__ void next_unit(const syn_paged_attn_args& a) {
+  __device__ __forceinline__ void next_unit(const syn_paged_attn_args& a, int heads) {
     step = 0;
-    if (++sub < a.Hkv * r.rt) return;
+    if (++sub < heads * r.rt) return;
     sub = 0;
     do {
       ++z;
@@ -413,6 +421,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   const syn_paged_attn_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int group = a.Hq / a.Hkv;
+  // Workers are teams of `tracks` warps, a warp for a track: head sub / rt * tracks + track.  On the line a group of
+  // `tracks` heads counts as one.
+  const int heads = a.Hkv / p.tracks, wide = PA_WARPS / p.tracks, team = warp / p.tracks, track = warp % p.tracks;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this warp's share of the line
@@ -421,7 +432,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   long long mine = 0;
   for (int z = z0; z < z1; ++z) {
     const PagedRequest r = paged_request<C>(a, z);
-    mine += static_cast<long long>(r.steps) * a.Hkv * r.rt;
+    mine += static_cast<long long>(r.steps) * heads * r.rt;
     if (blockIdx.x == 0) {
       if (a.lens[z] < 0) paged_record(a.status, SYN_DEV_BAD_INDEX, z, a.lens[z]);
       if (a.starts != nullptr && (a.starts[z] < 0 || a.starts[z + 1] < a.starts[z] || a.starts[z + 1] > a.tokens))
@@ -440,8 +451,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     if (w < warp) upto += s_sum[w];
     total += s_sum[w];
   }
-  const int shares = static_cast<int>(min(static_cast<long long>(p.grid) * PA_WARPS, max(1LL, total / p.min_steps)));
-  constexpr int wide = PA_WARPS;
+  const int shares = static_cast<int>(min(static_cast<long long>(p.grid) * wide, max(1LL, total / p.min_steps)));
   const PagedCut cut(total, shares);
 #pragma unroll
   for (int w = 0; w < PA_WARPS; ++w) {
@@ -452,7 +462,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       int z = z0;
       for (; z < z1; ++z) {
         const PagedRequest r = paged_request<C>(a, z);
-        const long long n = static_cast<long long>(r.steps) * a.Hkv * r.rt;
+        const long long n = static_cast<long long>(r.steps) * heads * r.rt;
         if (rest < n) break;
         rest -= n;
       }
@@ -463,8 +473,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   __syncthreads();  // from here on the warps go their own ways
   // Every warp has a record: those without work one of nothing to join.
   int32_t* const record = p.desc + (blockIdx.x * PA_WARPS + warp) * PA_DESC;
-  const int worker = blockIdx.x * wide + warp;
-  const bool works = warp < wide && worker < shares;
+  const int worker = blockIdx.x * wide + team;
+  const bool works = worker < shares;
   const long long t0 = works ? cut.at(worker) : total;
   const long long t1 = works ? cut.at(worker + 1) : total;
   PagedJoin join;
@@ -475,7 +485,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   }
 
   PagedCursor<C> cur;
-  cur.at(a, s_z[warp], s_rest[warp]);
+  cur.at(a, s_z[team], s_rest[team]);
   const long long unit0 = t0 - cur.step, unit1 = unit0 + cur.r.steps;  // the first unit, on the line
   // A block all of whose shares lie in one unit joins its warps' parts itself.
   auto pooled = [&](int block) {
@@ -499,7 +509,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       join.n3 = pool_last ? 0 : last - join.w3 + 1;
     }
     const int head = cur.sub / cur.r.rt;
-    join.s0 = cur.r.s0, join.kv_head = head, join.row0 = (cur.sub - head * cur.r.rt) * C::ROWS;
+    join.s0 = cur.r.s0, join.kv_head = head * p.tracks + track, join.row0 = (cur.sub - head * cur.r.rt) * C::ROWS;
     join.rows = min(C::ROWS, cur.r.n * group - join.row0);
   }
   if (lane == 0) {
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   PagedCursor<C> ahead = cur;
   int left = static_cast<int>(t1 - t0);  // steps that are yet to be asked for
   int page = -2, inside = 0;  // page of key (lane % KEYS) of the next step (-2: no such key), slot in it
-  int head_ahead = ahead.sub / ahead.r.rt;
+  int head_ahead = ahead.sub / ahead.r.rt * p.tracks + track;
   constexpr int EB = C::E4M3 ? 1 : 2, RPI = 32 / C::CPR, LOADS = C::KEYS / RPI;
   auto look_up = [&]() {
     page = -2;
@@ -568,8 +578,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       if (values) {
         --left;
         if (++ahead.step == ahead.r.steps) {
-          if (left > 0) ahead.next_unit(a);
-          head_ahead = ahead.sub / ahead.r.rt;
+          if (left > 0) ahead.next_unit(a, heads);
+          head_ahead = ahead.sub / ahead.r.rt * p.tracks + track;
         }
         look_up();
       }
@@ -598,36 +608,42 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   while (t < t1) {
     // ---- a unit: rows row0 .. row0 + rows of head kv_head of request z
     const PagedRequest r = cur.r;
-    const int kv_head = cur.sub / r.rt, row0 = (cur.sub - kv_head * r.rt) * C::ROWS;
+    const int head_group = cur.sub / r.rt, kv_head = head_group * p.tracks + track, row0 = (cur.sub - head_group * r.rt) * C::ROWS;
     const int rows = min(C::ROWS, r.n * group - row0);
     const int pos0 = r.len - r.n;
     const bool one = r.n == 1;  // one new token: spares the divisions
     const int steps = static_cast<int>(min(static_cast<long long>(r.steps - cur.step), t1 - t));
     // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
     // Rows behind the last repeat it.
-    int lo[2 * RT], hi[2 * RT];
-    float mult[2 * RT];
+    int pos[2 * RT];
 #pragma unroll
     for (int x = 0; x < 2 * RT; ++x) {
       const int tok = one ? 0 : (row0 + min((x >> 1) * 8 + 2 * t4 + (x & 1), rows - 1)) / group;
-      hi[x] = a.causal ? min(r.len, pos0 + tok + 1) : r.len;
-      lo[x] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
-      mult[x] = a.sm_scale * CUDART_L2E_F;
-      if constexpr (C::E4M3) mult[x] *= a.k_scale[kv_head];
+      pos[x] = pos0 + tok;
     }
+    // Keys lo .. hi - 1 are seen from position `at`.
+    auto lo = [&](int at) { return a.window > 0 ? at - a.window + 1 : 0; };
+    auto hi = [&](int at) { return a.causal ? min(r.len, at + 1) : r.len; };
+    // From product to power of two; a key that is not seen gets the product that stands for a power of -inf, so the
+    // factor must not be 0 (which 1e-30 stands for: scores then differ by less than a rounding).
+    float mult = a.sm_scale * CUDART_L2E_F;
+    if constexpr (C::E4M3) mult *= a.k_scale[kv_head];
+    if (fabsf(mult) < 1e-30f) mult = 1e-30f;
+    const float unseen = mult > 0.f ? -CUDART_INF_F : CUDART_INF_F;
     const T* qrow[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int row = row0 + min(8 * i + g, rows - 1), tok = one ? 0 : row / group, head = kv_head * group + row - tok * group;
       qrow[i] = static_cast<const T*>(a.q) + static_cast<int64_t>(r.s0 + tok) * a.q_strides[0] + head * a.q_strides[1];
     }
-    const int tok_a = one ? 0 : row0 / group, tok_b = one ? 0 : (row0 + rows - 1) / group;
-    const int all_lo = a.window > 0 ? max(0, pos0 + tok_b - a.window + 1) : 0;  // keys that every row sees
-    const int all_hi = a.causal ? min(r.len, pos0 + tok_a + 1) : r.len;
+    const int all_lo = lo(pos0 + (one ? 0 : (row0 + rows - 1) / group));  // keys that every row sees
+    const int all_hi = hi(pos0 + (one ? 0 : row0 / group));
 
     // ---- query fragments
-    float up[RT];  // bf16 queries over 8-bit keys: a power of two brings each row into the range of halves
-    if constexpr (C::E4M3 && BF16) {
+    // bf16 queries over 8-bit keys: a power of two brings each row into the range of halves.
+    constexpr bool SHIFT = C::E4M3 && BF16;
+    float up[RT], down[SHIFT ? 2 * RT : 1] = {};
+    if constexpr (SHIFT) {
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         uint32_t top = 0;  // largest magnitude as bits
@@ -643,11 +659,12 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
         const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
         up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+        const float back = mult * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) mult[2 * i + c] *= __shfl_sync(~0u, down, (2 * t4 + c) * 4);
+        for (int c = 0; c < 2; ++c) down[2 * i + c] = __shfl_sync(~0u, back, (2 * t4 + c) * 4);
       }
     }
+    auto factor = [&](int x) { return SHIFT ? down[SHIFT ? x : 0] : mult; };
     auto q_frag = [&](int ks, int i, uint32_t (&f)[2]) {
       if constexpr (!C::E4M3) {
         f[0] = __ldg(reinterpret_cast<const uint32_t*>(qrow[i]) + ks * 8 + t4);
@@ -690,9 +707,10 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       }
     };
 
-    float o[C::DT][RT][4], m[2 * RT], slack[2 * RT], l[2 * RT];
+    // A row without a key so far has the reference PA_NONE, from which any score is a rise.
+    float o[C::DT][RT][4], m[2 * RT], l[2 * RT];
 #pragma unroll
-    for (int x = 0; x < 2 * RT; ++x) m[x] = 0.f, slack[x] = -CUDART_INF_F, l[x] = 0.f;  // slack: the reference may stay that far behind
+    for (int x = 0; x < 2 * RT; ++x) m[x] = PA_NONE, l[x] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
@@ -726,7 +744,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int j = 0; j < RT; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) s2[j][c] = 0.f;
-        constexpr int GROUP = C::KSTEPS < 8 ? C::KSTEPS : 8;
+        constexpr int GROUP = C::KSTEPS < 8 || RT > 1 ? 4 : 8;
 #pragma unroll
         for (int k0 = 0; k0 < C::KSTEPS; k0 += GROUP) {
           uint32_t k[GROUP][4];
@@ -750,24 +768,25 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       } else {
 #pragma unroll
         for (int part = 0; part < C::D / 64; ++part) {
-          uint32_t f[4][RT][2];
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int j = 0; j < RT; ++j) q_at(part * 4 + w, j, f[w][j]);
+          uint4 x[SN], y[SN];
 #pragma unroll
           for (int n = 0; n < SN; ++n) {
             const uint32_t at = k_at + ring_at<C, false>(g, t4 + part * 4) + n * 16 * C::ROWB;
-            const uint4 x = lds16(at), y = lds16(at + 8 * C::ROWB);
-            if (part == 0 && n == 0) refill(false);  // its arithmetic fills the wait for the keys
-            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+            x[n] = lds16(at), y[n] = lds16(at + 8 * C::ROWB);
+          }
+          if (part == 0) refill(false);  // its arithmetic fills the wait for the keys
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 4; ++w) {
+            uint32_t f[RT][2];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) q_at(part * 4 + w, j, f[j]);
+#pragma unroll
+            for (int n = 0; n < SN; ++n) {
               uint32_t k[4];
-              e4m3x4_to_h2x2(xw[w], k[0], k[2]);
-              e4m3x4_to_h2x2(yw[w], k[1], k[3]);
+              e4m3x4_to_h2x2(reinterpret_cast<const uint32_t*>(&x[n])[w], k[0], k[2]);
+              e4m3x4_to_h2x2(reinterpret_cast<const uint32_t*>(&y[n])[w], k[1], k[3]);
 #pragma unroll
-              for (int j = 0; j < RT; ++j) mma16816<false>(s[n][j], k, f[w][j][0], f[w][j][1]);
+              for (int j = 0; j < RT; ++j) mma16816<false>(s[n][j], k, f[j][0], f[j][1]);
             }
           }
         }
@@ -775,44 +794,46 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
       // ---- weights
       const bool whole = base >= all_lo && base + C::KEYS <= all_hi;  // every row sees every key
-      float y[SN][RT][4];  // score minus reference, in powers of two
+      if (!whole) {
+#pragma unroll
+        for (int x = 0; x < 2 * RT; ++x) {
+          const int from = lo(pos[x]), to = hi(pos[x]);
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = base + n * 16 + h * 8 + g;
+              if (key < from || key >= to) s[n][x >> 1][2 * h + (x & 1)] = unseen;
+            }
+        }
+      }
       bool rise = false;
 #pragma unroll
       for (int x = 0; x < 2 * RT; ++x)
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = 2 * h + (x & 1), key = base + n * 16 + h * 8 + g;
-            float& v = y[n][x >> 1][c];
-            v = fmaf(s[n][x >> 1][c], mult[x], -m[x]);
-            if (!whole && (key < lo[x] || key >= hi[x])) v = -CUDART_INF_F;
-            rise |= v > slack[x];
-          }
+          for (int h = 0; h < 2; ++h) rise |= fmaf(s[n][x >> 1][2 * h + (x & 1)], factor(x), -m[x]) > PA_SLACK;
       if (__any_sync(~0u, rise)) {
 #pragma unroll
         for (int x = 0; x < 2 * RT; ++x) {
           float top = -CUDART_INF_F;
 #pragma unroll
-          for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(y[n][x >> 1][x & 1], y[n][x >> 1][2 + (x & 1)]));
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) top = fmaxf(top, s[n][x >> 1][2 * h + (x & 1)] * factor(x));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-          const bool none = slack[x] == -CUDART_INF_F;  // no key so far: any reference will do
-          if (top > (none ? -CUDART_INF_F : 0.f)) {
-            const float by = m[x] + top - m[x], alpha = none ? 0.f : ex2(-by);
-            m[x] += top;
-            slack[x] = PA_SLACK;
+          if (top > m[x]) {
+            const float alpha = ex2(m[x] - top);
+            m[x] = top;
             l[x] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < C::DT; ++dt) {
               o[dt][x >> 1][x & 1] *= alpha;
               o[dt][x >> 1][2 + (x & 1)] *= alpha;
             }
-#pragma unroll
-            for (int n = 0; n < SN; ++n)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) y[n][x >> 1][2 * h + (x & 1)] -= by;
           }
         }
       }
@@ -822,8 +843,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float& v = y[n][x >> 1][2 * h + (x & 1)];
-            v = ex2(v);
+            float& v = s[n][x >> 1][2 * h + (x & 1)];
+            v = ex2(fmaf(v, factor(x), -m[x]));
             l[x] += v;
           }
       const uint32_t v_at = ready();
@@ -838,7 +859,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         for (int j = 0; j < RT; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float w0 = y[kk][j][2 * h], w1 = y[kk][j][2 * h + 1];
+            const float w0 = s[kk][j][2 * h], w1 = s[kk][j][2 * h + 1];
             const uint32_t top = pack2<MBF16>(w0, w1);
             ph[j][h] = transpose8(top);
             const float2 b = unpack2<MBF16>(top);
@@ -869,7 +890,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
             const int j = x >> 1;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {  // row 8 j + 2 q + (x & 1), a column of lanes t4 == q
-              const int row_lo = __shfl_sync(~0u, lo[x], q), row_hi = __shfl_sync(~0u, hi[x], q);
+              const int at = __shfl_sync(~0u, pos[x], q), row_lo = lo(at), row_hi = hi(at);
               const int key = base + kk * 16 + t4 * 2;
               auto seen = [&](int k) {
                 return (k >= row_lo && k < row_hi ? 0xFFFFu : 0u) | (k + 1 >= row_lo && k + 1 < row_hi ? 0xFFFF0000u : 0u);
@@ -893,19 +914,19 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 
     // ---- the unit, or this worker's part of it, is done
     const bool from_start = cur.step == 0, to_end = cur.step + steps == r.steps, partial = !(from_start && to_end);
-    const int part = 2 * worker + (first_segment ? 0 : 1);
+    const int part = (2 * worker + (first_segment ? 0 : 1)) * p.tracks + track;
 #pragma unroll
     for (int x = 0; x < 2 * RT; ++x) {
       l[x] += __shfl_xor_sync(~0u, l[x], 4);
       l[x] += __shfl_xor_sync(~0u, l[x], 8);
       l[x] += __shfl_xor_sync(~0u, l[x], 16);
-      if (slack[x] == -CUDART_INF_F) m[x] = -CUDART_INF_F;
+      if (m[x] == PA_NONE) m[x] = -CUDART_INF_F;
     }
     if (pool) {
       // The warps' parts meet in shared memory, in place of the rings, and each warp joins some fragments.
       cp_async_wait<0>();
       __syncwarp();
-      const int active = min(wide, shares - static_cast<int>(blockIdx.x) * wide);
+      const int active = min(wide, shares - static_cast<int>(blockIdx.x) * wide);  // teams
       auto own_o = [&](int w) { return reinterpret_cast<float4*>(smem + w * C::RING) + lane; };
       auto own_ml = [&](int w) { return reinterpret_cast<float4*>(smem + w * C::RING + C::FRAGS * 512) + lane; };
 #pragma unroll
@@ -915,19 +936,19 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
           own_o(warp)[(dt * RT + j) * 32] = make_float4(o[dt][j][0], o[dt][j][1], o[dt][j][2], o[dt][j][3]);
         own_ml(warp)[j * 32] = make_float4(m[2 * j], l[2 * j], m[2 * j + 1], l[2 * j + 1]);
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(active * 32) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"r"(active * p.tracks * 32) : "memory");
       const bool all = unit0 == cut.at(blockIdx.x * wide) &&
                        unit1 == cut.at(min((static_cast<int>(blockIdx.x) + 1) * wide, shares));
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) * wide;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) * wide * p.tracks + track;
 #pragma unroll 1
-      for (int f = warp; f < C::FRAGS; f += active) {
+      for (int f = team; f < C::FRAGS; f += active) {
         const int dt = f / RT, j = f % RT;
         PagedSum<1> sum;
         sum.clear();
 #pragma unroll 1
         for (int w = 0; w < active; ++w) {
-          const float4 u[1] = {own_o(w)[f * 32]};
-          sum.add(own_ml(w)[j * 32], u);
+          const float4 u[1] = {own_o(w * p.tracks + track)[f * 32]};
+          sum.add(own_ml(w * p.tracks + track)[j * 32], u);
         }
         if (j * 8 >= rows) continue;
         if (all) {
@@ -967,7 +988,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     }
     first_segment = false;
     t += steps;
-    if (t < t1) cur.next_unit(a);
+    if (t < t1) cur.next_unit(a, heads);
   }
 }
 

@@ -2,9 +2,16 @@
 // compute).
 #include "paged.cuh"
 
+#include <atomic>
+#include <type_traits>
+
 namespace syn {
 
+// The plan is short work on a few tables: its time is that of its dependent steps.  Up to a few thousand tokens one
+// block does it; the slots of more are dealt out to a cluster, whose blocks all run the same sums.
 constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_CLUSTER = 8;
+constexpr int PLAN_ALONE = 4096;  // tokens
 
 struct PlanSums {
   long long given, want, more;  // pages pushed, pages popped, tokens appended
@@ -17,9 +24,10 @@ __device__ __forceinline__ PlanSums shfl_up(PlanSums a, int d) {
   return {__shfl_up_sync(~0u, a.given, d), __shfl_up_sync(~0u, a.want, d), __shfl_up_sync(~0u, a.more, d)};
 }
 
-// One block: running sums over the requests give every request its place on the stack of free pages
-// and its first token; then pages are pushed, popped and the tokens' slots written.
-__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_args p) {
+// Running sums over the requests give every request its place on the stack of free pages and its first token; then
+// pages are pushed, popped and the tokens' slots written.  BLOCKS = blocks of the only cluster.
+template <int BLOCKS>
+__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_constant__ syn_page_plan_args p) {
   extern __shared__ int32_t plan_smem[];
   int32_t* s_lens = plan_smem;                  // [requests]
   int32_t* s_given = s_lens + p.requests;       // pages pushed before the request; -1: the request goes on
@@ -27,28 +35,33 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
   int32_t* s_start = s_want + p.requests;       // [requests + 1]
   __shared__ PlanSums warp_sums[32];
   __shared__ int s_bad;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  const int block = BLOCKS == 1 ? 0 : blockIdx.x;
   if (tid == 0) s_bad = INT_MAX;
   __syncthreads();
 
-  const int per = (p.requests + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int per = (p.requests + threads - 1) / threads;
   const int z0 = min(tid * per, p.requests), z1 = min(z0 + per, p.requests);
   const long long room = static_cast<long long>(p.width) * p.page_size;
-  auto sums_of = [&](int len, int add) {
-    const int held = (static_cast<long long>(len) + p.page_size - 1) / p.page_size;
+  const uint32_t page_size = p.page_size;
+  auto pages_of = [&](uint32_t n) { return n / page_size + (n % page_size != 0); };
+  auto sums_of = [&](int len, int add) {  // len + add is at most width * page_size, or the request is refused
+    const int held = pages_of(len);
     PlanSums s = {0, 0, 0};
     if (add < 0) {
       s.given = held;
     } else {
-      s.want = (static_cast<long long>(len) + add + p.page_size - 1) / p.page_size - held;
+      s.want = pages_of(static_cast<uint32_t>(len) + add) - held;
       s.more = add;
     }
     return s;
   };
+  const int top0 = p.num_free[0];
   PlanSums mine = {0, 0, 0};
   for (int z = z0; z < z1; ++z) {
     const int len = p.lens[z], add = p.add[z];
     s_lens[z] = len;
+    s_given[z] = add;
     if (len < 0 || static_cast<long long>(len) + max(add, 0) > room) {
       atomicMin(&s_bad, z);
     } else {
@@ -63,7 +76,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
   if (lane == 31) warp_sums[warp] = upto;
   __syncthreads();
   if (warp == 0) {
-    PlanSums w = warp_sums[lane];
+    PlanSums w = lane < warps ? warp_sums[lane] : PlanSums{0, 0, 0};
     for (int d = 1; d < 32; d <<= 1) {
       const PlanSums o = shfl_up(w, d);
       if (lane >= d) w = w + o;
@@ -74,14 +87,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
   const PlanSums total = warp_sums[31];
   PlanSums at = upto;
   if (warp > 0) at = at + warp_sums[warp - 1];
-  const int top0 = p.num_free[0];
   const long long top = top0 + total.given;
 
   const bool range = s_bad != INT_MAX || top0 < 0 || top0 > p.num_pages || top > p.num_pages || total.more > p.tokens;
   const bool refused = range || total.want > top;
   at.given -= mine.given, at.want -= mine.want, at.more -= mine.more;
   for (int z = z0; z < z1; ++z) {
-    const int len = s_lens[z], add = p.add[z];
+    const int len = s_lens[z], add = s_given[z];
     if (!refused) {
       s_given[z] = add < 0 ? static_cast<int>(at.given) : -1;
       s_want[z] = static_cast<int>(at.want);
@@ -92,44 +104,54 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
     }
   }
   if (tid == 0) s_start[p.requests] = refused ? 0 : static_cast<int>(total.more);
-  __syncthreads();  // after this nobody reads lens, add or num_free again: the outputs may be the inputs
+  __syncthreads();
 
+  const int first = block * warps + warp, skip = BLOCKS * warps;  // a warp takes a request
+  if (!refused && total.given > 0) {
+    for (int z = first; z < p.requests; z += skip) {
+      if (s_given[z] < 0) continue;
+      const int held = pages_of(s_lens[z]);
+      for (int j = lane; j < held; j += 32) p.free_pages[top0 + s_given[z] + j] = p.table[z * p.table_stride + j];
+    }
+  }
+  // Pages pushed are seen by all, and nobody reads lens, add or num_free again: the outputs may be the inputs.
+  if constexpr (BLOCKS == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   if (refused) {
-    if (tid == 0) {
+    if (block == 0 && tid == 0) {
       if (range) {
         paged_record(p.status, SYN_DEV_BAD_INDEX, s_bad != INT_MAX ? s_bad : -1, s_bad != INT_MAX ? s_lens[s_bad] : top0);
       } else {
         paged_record(p.status, SYN_DEV_NO_PAGES, -1, static_cast<int>(min(total.want, static_cast<long long>(INT_MAX))));
       }
     }
-  } else {
-    for (int z = warp; z < p.requests; z += PLAN_THREADS / 32) {
-      if (s_given[z] < 0) continue;
-      const int held = (s_lens[z] + p.page_size - 1) / p.page_size;
-      for (int j = lane; j < held; j += 32) p.free_pages[top0 + s_given[z] + j] = p.table[z * p.table_stride + j];
-    }
-    __syncthreads();
-    for (int z = warp; z < p.requests; z += PLAN_THREADS / 32) {
+  } else if (total.want > 0) {
+    for (int z = first; z < p.requests; z += skip) {
       if (s_given[z] >= 0) continue;
-      const int held = (s_lens[z] + p.page_size - 1) / p.page_size;
+      const int held = pages_of(s_lens[z]);
       const int want = (z + 1 < p.requests ? s_want[z + 1] : static_cast<int>(total.want)) - s_want[z];
       for (int j = lane; j < want; j += 32)
-        p.table[z * p.table_stride + held + j] = p.free_pages[top - 1 - s_want[z] - j];
+        p.table[z * p.table_stride + held + j] = __ldcg(p.free_pages + top - 1 - s_want[z] - j);
     }
-    __syncthreads();
   }
-  for (int t = tid; t < p.tokens; t += PLAN_THREADS) {
+  const int tokens = s_start[p.requests];
+  for (int t = block * threads + tid; t < p.tokens; t += BLOCKS * threads) {
     int slot = -1, position = 0;
-    if (t < s_start[p.requests]) {
+    if (t < tokens) {
       int a = 0, b = p.requests;  // the last request that starts at or before t
       while (b - a > 1) {
         const int m = (a + b) >> 1;
         (s_start[m] <= t ? a : b) = m;
       }
       position = s_lens[a] + t - s_start[a];
-      const int page = p.table[a * p.table_stride + position / p.page_size];
+      const int i = position / page_size, held = pages_of(s_lens[a]);
+      // A page that the request had is in the table; a new one is read where it comes from, not where another warp puts it.
+      const int page = i < held ? p.table[a * p.table_stride + i] : __ldcg(p.free_pages + top - 1 - s_want[a] - (i - held));
       if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) {
-        slot = page * p.page_size + position % p.page_size;
+        slot = page * p.page_size + position % page_size;
       } else {
         paged_record(p.status, SYN_DEV_BAD_INDEX, a, page);
       }
@@ -137,12 +159,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
     p.slots[t] = slot;
     if (p.positions != nullptr) p.positions[t] = position;
   }
-  for (int z = tid; z < p.requests; z += PLAN_THREADS) {
+  if (block != 0) return;
+  for (int z = tid; z < p.requests; z += threads) {
     p.starts[z] = s_start[z];
     p.lens_out[z] = refused ? s_lens[z] : s_given[z] >= 0 ? 0 : s_lens[z] + s_start[z + 1] - s_start[z];
   }
   if (tid == 0) {
-    p.starts[p.requests] = s_start[p.requests];
+    p.starts[p.requests] = tokens;
     p.num_free_out[0] = refused ? top0 : static_cast<int>(top - total.want);
   }
 }
@@ -150,73 +173,132 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(syn_page_plan_a
 // ----------------------------------------------------------------------------- append
 constexpr int APPEND_THREADS = 256;
 
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ float2 pair_to_float(uint32_t x) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ uint32_t e4m3_pair(float x, float y) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+}
 
-// One thread moves 16 elements of one head.
-template <typename T, bool E4M3>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(syn_paged_append_args p) {
-  const int parts = p.D / 16;
-  const long long items = static_cast<long long>(p.tokens) * 2 * p.Hkv * parts;
-  const long long i = static_cast<long long>(blockIdx.x) * APPEND_THREADS + threadIdx.x;
-  if (i >= items) return;
-  const int part = static_cast<int>(i % parts);
-  const int h = static_cast<int>(i / parts % p.Hkv);
-  const int which = static_cast<int>(i / parts / p.Hkv % 2);
-  const int t = static_cast<int>(i / parts / p.Hkv / 2);
-  const int slot = p.slots[t];
-  if (slot < 0) return;
-  if (slot >= p.num_pages * p.page_size) {
-    paged_record(p.status, SYN_DEV_BAD_INDEX, t, slot);
-    return;
+// Eight elements of one head are an item.  A thread has one item of a token, whose place it works out once, and moves
+// it for TOKENS tokens, all of which it has on the way before the first is stored.
+template <typename T, bool E4M3, int TOKENS>
+__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __grid_constant__ syn_paged_append_args p) {
+  const int parts = p.D / 8, items = 2 * p.Hkv * parts;
+  const int at_once = items < APPEND_THREADS ? APPEND_THREADS / items : 1;  // tokens that a block moves side by side
+  const int width = items < APPEND_THREADS ? items : APPEND_THREADS;
+  const int side = threadIdx.x / width, item = blockIdx.y * APPEND_THREADS + threadIdx.x % width;
+  if (side >= at_once || item >= items) return;
+  const int part = item % parts, h = item / parts % p.Hkv;
+  const bool values = item >= p.Hkv * parts;
+  const int64_t row = values ? p.v_strides[0] : p.k_strides[0];
+  const T* x = static_cast<const T*>(values ? p.v : p.k) + h * (values ? p.v_strides[1] : p.k_strides[1]) + part * 8;
+  const int64_t place = h * p.cache_strides[2] + part * 8;
+  void* cache = values ? p.v_cache : p.k_cache;
+  const int t0 = blockIdx.x * (at_once * TOKENS) + side;
+  int slot[TOKENS];
+  uint4 v[TOKENS];
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    const int t = t0 + i * at_once;
+    slot[i] = t < p.tokens ? __ldg(p.slots + t) : -1;
   }
-  const int64_t* xs = which ? p.v_strides : p.k_strides;
-  const T* x = static_cast<const T*>(which ? p.v : p.k) + t * xs[0] + h * xs[1] + part * 16;
-  const int64_t at = slot / p.page_size * p.cache_strides[0] + slot % p.page_size * p.cache_strides[1] +
-                     h * p.cache_strides[2] + part * 16;
-  const uint4 a = reinterpret_cast<const uint4*>(x)[0], b = reinterpret_cast<const uint4*>(x)[1];
-  if constexpr (E4M3) {
-    const float scale = (which ? p.v_scale : p.k_scale)[h];
-    uint4 packed;
-    unsigned char* out = reinterpret_cast<unsigned char*>(&packed);
-    const T* in = reinterpret_cast<const T*>(&a);
-    const T* in2 = reinterpret_cast<const T*>(&b);
-    for (int j = 0; j < 8; ++j) {
-      out[j] = __nv_cvt_float_to_fp8(__fdiv_rn(to_float(in[j]), scale), __NV_SATFINITE, __NV_E4M3);
-      out[8 + j] = __nv_cvt_float_to_fp8(__fdiv_rn(to_float(in2[j]), scale), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i)
+    if (slot[i] >= 0) v[i] = __ldg(reinterpret_cast<const uint4*>(x + (t0 + i * at_once) * row));
+  float scale = 1.f;
+  if constexpr (E4M3) scale = (values ? p.v_scale : p.k_scale)[h];
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    if (slot[i] < 0) continue;
+    const uint32_t page = static_cast<uint32_t>(slot[i]) / static_cast<uint32_t>(p.page_size);
+    if (page >= static_cast<uint32_t>(p.num_pages)) {
+      paged_record(p.status, SYN_DEV_BAD_INDEX, t0 + i * at_once, slot[i]);
+      continue;
     }
-    *reinterpret_cast<uint4*>(static_cast<unsigned char*>(which ? p.v_cache : p.k_cache) + at) = packed;
-  } else {
-    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(which ? p.v_cache : p.k_cache) + at);
-    out[0] = a;
-    out[1] = b;
+    const int64_t at = page * p.cache_strides[0] + (slot[i] - static_cast<int>(page) * p.page_size) * p.cache_strides[1] + place;
+    if constexpr (E4M3) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = pair_to_float<T>(w[j]);
+        q[j] = e4m3_pair(__fdiv_rn(f.x, scale), __fdiv_rn(f.y, scale));
+      }
+      *reinterpret_cast<uint2*>(static_cast<unsigned char*>(cache) + at) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<T*>(cache) + at) = v[i];
+    }
   }
 }
 
+template <typename T, bool E4M3>
 static int launch_append(const syn_paged_append_args& a, cudaStream_t stream) {
-  const long long items = static_cast<long long>(a.tokens) * 2 * a.Hkv * (a.D / 16);
-  const unsigned grid = static_cast<unsigned>((items + APPEND_THREADS - 1) / APPEND_THREADS);
-  const bool bf16 = a.dtype == SYN_DTYPE_BF16;
-  if (a.cache_dtype == SYN_CACHE_E4M3) {
-    if (bf16) paged_append_kernel<__nv_bfloat16, true><<<grid, APPEND_THREADS, 0, stream>>>(a);
-    else paged_append_kernel<__half, true><<<grid, APPEND_THREADS, 0, stream>>>(a);
-  } else {  // a copy of 16-bit words
-    paged_append_kernel<__half, false><<<grid, APPEND_THREADS, 0, stream>>>(a);
-  }
+  const int items = 2 * a.Hkv * (a.D / 8);
+  const int at_once = items < APPEND_THREADS ? APPEND_THREADS / items : 1;
+  const int columns = (items + APPEND_THREADS - 1) / APPEND_THREADS;
+  // Four tokens a thread where that still makes a few blocks for every SM: 64 bytes on the way a thread carry the
+  // stream; one where there are so few that latency counts.
+  const int64_t rows = (a.tokens + at_once - 1) / at_once;
+  const dim3 one(static_cast<unsigned>(rows), columns), four(static_cast<unsigned>((rows + 3) / 4), columns);
+  if (columns > 65535) return SYN_ERR_TOO_LARGE;
+  if (rows * columns >= 4096) paged_append_kernel<T, E4M3, 4><<<four, APPEND_THREADS, 0, stream>>>(a);
+  else paged_append_kernel<T, E4M3, 1><<<one, APPEND_THREADS, 0, stream>>>(a);
   SYN_CUDA_TRY(cudaGetLastError());
+  return SYN_OK;
+}
+
+template <typename T, bool E4M3>
+static int preload_append() {
+  cudaFuncAttributes attr;
+  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_append_kernel<T, E4M3, 1>));
+  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_append_kernel<T, E4M3, 4>));
   return SYN_OK;
 }
 
 constexpr int PLAN_SMEM_MAX = (4 * SYN_PAGE_PLAN_MAX_REQUESTS + 1) * 4;
 
-int preload_paged_kernels() {
-  cudaFuncAttributes attr;
-  SYN_CUDA_TRY(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM_MAX));
-  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, page_plan_kernel));
-  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_append_kernel<__half, false>));
-  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_append_kernel<__half, true>));
-  SYN_CUDA_TRY(cudaFuncGetAttributes(&attr, paged_append_kernel<__nv_bfloat16, true>));
+template <int BLOCKS>
+static int configure_plan() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  SYN_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return SYN_OK;
+  SYN_CUDA_TRY(cudaFuncSetAttribute(page_plan_kernel<BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM_MAX));
+  done.fetch_or(bit, std::memory_order_relaxed);
   return SYN_OK;
+}
+
+template <int BLOCKS>
+static int launch_plan(const syn_page_plan_args& a, int threads, cudaStream_t stream) {
+  const int rc = configure_plan<BLOCKS>();
+  if (rc != SYN_OK) return rc;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = BLOCKS, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(BLOCKS);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = (4 * a.requests + 1) * 4;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = BLOCKS > 1 ? 1 : 0;
+  SYN_CUDA_TRY(cudaLaunchKernelEx(&config, page_plan_kernel<BLOCKS>, a));
+  return SYN_OK;
+}
+
+int preload_paged_kernels() {
+  int rc = configure_plan<1>();
+  if (rc == SYN_OK) rc = configure_plan<PLAN_CLUSTER>();
+  if (rc == SYN_OK) rc = preload_append<__half, false>();
+  if (rc == SYN_OK) rc = preload_append<__half, true>();
+  if (rc == SYN_OK) rc = preload_append<__nv_bfloat16, true>();
+  return rc;
 }
 
 }  // namespace syn
@@ -233,12 +315,9 @@ extern "C" int syn_page_plan(const syn_page_plan_args* a, void* stream) {
   if (static_cast<int64_t>(a->num_pages) * a->page_size > INT_MAX) return SYN_ERR_TOO_LARGE;
   PagedDevice device(a->device);
   SYN_CUDA_TRY(device.error());
-  const int smem = (4 * a->requests + 1) * 4;
-  if (smem > 48 * 1024)
-    SYN_CUDA_TRY(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM_MAX));
-  page_plan_kernel<<<1, PLAN_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(*a);
-  SYN_CUDA_TRY(cudaGetLastError());
-  return SYN_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->tokens > PLAN_ALONE) return launch_plan<PLAN_CLUSTER>(*a, PLAN_THREADS, s);
+  return launch_plan<1>(*a, a->requests <= 256 && a->tokens <= 1024 ? 256 : PLAN_THREADS, s);
 }
 
 extern "C" int syn_paged_append(const syn_paged_append_args* a, void* stream) {
@@ -249,7 +328,7 @@ extern "C" int syn_paged_append(const syn_paged_append_args* a, void* stream) {
   if (a->cache_dtype != SYN_CACHE_SAME && a->cache_dtype != SYN_CACHE_E4M3) return SYN_ERR_UNSUPPORTED;
   if (a->D % 16 != 0) return SYN_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a->num_pages) * a->page_size > INT_MAX) return SYN_ERR_TOO_LARGE;
-  if (static_cast<int64_t>(a->tokens) * a->Hkv * (a->D / 16) > INT_MAX) return SYN_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(a->Hkv) * a->D > INT_MAX / 2) return SYN_ERR_TOO_LARGE;
   if (a->tokens == 0) return SYN_OK;
   syn_paged_append_args p = *a;
   const bool e4m3 = a->cache_dtype == SYN_CACHE_E4M3;
@@ -262,5 +341,7 @@ extern "C" int syn_paged_append(const syn_paged_append_args* a, void* stream) {
     return SYN_ERR_INVALID;
   PagedDevice device(a->device);
   SYN_CUDA_TRY(device.error());
-  return launch_append(p, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!e4m3) return launch_append<__half, false>(p, s);  // a copy of 16-bit words
+  return a->dtype == SYN_DTYPE_BF16 ? launch_append<__nv_bfloat16, true>(p, s) : launch_append<__half, true>(p, s);
 }
