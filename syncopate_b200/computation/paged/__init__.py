@@ -32,28 +32,32 @@ def _refuse(where: str, what: str):
     raise ValueError(f"{where}: {what}")
 
 
-def _check_ints(where: str, device, **tensors) -> None:
+# Devices are compared by ordinal (-1 = CPU): the calls are made once a layer and token, and a comparison of
+# torch.device objects takes several times as long.
+def _check_ints(where: str, index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t.dtype is not _INT or t.device != device or not t.is_contiguous():
-            _refuse(where, f"{name} must be a contiguous int32 tensor on {device}")
+        if t.dtype is not _INT or t.get_device() != index or not t.is_contiguous():
+            _refuse(where, f"{name} must be a contiguous int32 tensor on the device of the others")
 
 
-def _check_status(where: str, device, status) -> int:
+def _check_status(where: str, index: int, status) -> int:
     if status is None:
         return 0
     if isinstance(status, int):
         return status
-    if status.dtype is not _INT or status.device != device or status.numel() < 4 or not status.is_contiguous():
-        _refuse(where, f"status must be four int32 words on {device}")
+    if status.dtype is not _INT or status.get_device() != index or status.numel() < 4 or not status.is_contiguous():
+        _refuse(where, "status must be four int32 words on the device of the others")
     return status.data_ptr()
 
 
-def _check_table(where: str, device, table) -> int:
+def _check_table(where: str, index: int, table) -> int:
     """The row stride of a block table."""
-    if table.dtype is not _INT or table.device != device or table.dim() != 2 or table.stride(1) != 1:
-        _refuse(where, f"table must be an int32 [requests, width] tensor on {device} with unit inner stride")
+    if table.dtype is not _INT or table.get_device() != index or table.dim() != 2:
+        _refuse(where, "table must be an int32 [requests, width] tensor on the device of the others")
     rows, width = table.shape
-    stride = table.stride(0)
+    stride, inner = table.stride()
+    if inner != 1 and width > 1:
+        _refuse(where, "table must have unit inner stride")
     if stride < width:
         if rows > 1:
             _refuse(where, "the rows of table overlap")
@@ -76,7 +80,7 @@ def _check_cache(where: str, k_cache, v_cache, dtype, k_scale, v_scale):
     if k_cache.stride(3) != 1 and k_cache.shape[3] > 1:
         _refuse(where, "the head dimension of the caches must be contiguous")
     kept = k_cache.dtype
-    if kept is not v_cache.dtype or k_cache.device != v_cache.device:
+    if kept is not v_cache.dtype or k_cache.get_device() != v_cache.get_device():
         _refuse(where, "k_cache and v_cache must agree in type and device")
     if kept is dtype:
         if k_scale is not None or v_scale is not None:
@@ -85,7 +89,7 @@ def _check_cache(where: str, k_cache, v_cache, dtype, k_scale, v_scale):
     if kept is not torch.float8_e4m3fn:
         _refuse(where, f"the caches must be {dtype} or torch.float8_e4m3fn, not {kept}")
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if (t is None or t.dtype is not torch.float32 or t.device != k_cache.device or t.dim() != 1
+        if (t is None or t.dtype is not torch.float32 or t.get_device() != k_cache.get_device() or t.dim() != 1
                 or t.shape[0] != k_cache.shape[2] or not t.is_contiguous()):
             _refuse(where, f"an 8-bit cache needs {name}, a float32 tensor with one value a head")
     return L.SYN_CACHE_E4M3, k_scale.data_ptr(), v_scale.data_ptr()
@@ -116,11 +120,11 @@ def page_plan(
     ``num_free_out`` are given.  Apart from that no two tensors may overlap.  A step that does not fit
     changes nothing, gives no slots, and is told in ``status``."""
     where = "page_plan"
-    device = lens.device
+    index = lens.get_device()
     lens_out = lens if lens_out is None else lens_out
     num_free_out = num_free if num_free_out is None else num_free_out
-    table_stride = _check_table(where, device, table)
-    _check_ints(where, device, lens=lens, add=add, free_pages=free_pages, num_free=num_free, slots=slots, starts=starts,
+    table_stride = _check_table(where, index, table)
+    _check_ints(where, index, lens=lens, add=add, free_pages=free_pages, num_free=num_free, slots=slots, starts=starts,
                 lens_out=lens_out, num_free_out=num_free_out)
     requests, width = table.shape
     if (lens.numel(), add.numel(), starts.numel(), lens_out.numel()) != (requests, requests, requests + 1, requests):
@@ -128,20 +132,19 @@ def page_plan(
     if num_free.numel() != 1 or num_free_out.numel() != 1:
         _refuse(where, "num_free holds one number")
     if positions is not None:
-        _check_ints(where, device, positions=positions)
+        _check_ints(where, index, positions=positions)
         if positions.numel() != slots.numel():
             _refuse(where, "positions and slots must have the same length")
     if page_size <= 0:
         _refuse(where, "page_size must be positive")
-    if not lens.is_cuda:
+    if index < 0:
         _refuse(where, "the tensors must be on a CUDA device")
     if requests == 0:
         _refuse(where, "table has no rows")
-    index = device.index
     args = L.pack_page_plan(
         lens.data_ptr(), add.data_ptr(), table.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), slots.data_ptr(),
         0 if positions is None else positions.data_ptr(), starts.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(),
-        _check_status(where, device, status), table_stride, requests, width, page_size, free_pages.numel(),
+        _check_status(where, index, status), table_stride, requests, width, page_size, free_pages.numel(),
         slots.numel(), index)
     rc = L.lib().syn_page_plan(args, _stream(index, stream))
     if rc:
@@ -168,40 +171,40 @@ def paged_append(
     where = "paged_append"
     if k.dtype not in _DTYPES or v.dtype is not k.dtype:
         _refuse(where, "k and v must be fp16/bf16 tensors of one type")
-    device = k.device
-    if k.dim() != 3 or k.shape != v.shape or v.device != device:
+    index = k.get_device()
+    if k.dim() != 3 or k.shape != v.shape or v.get_device() != index:
         _refuse(where, "k and v must be [tokens, heads, dim] tensors of one shape and device")
     tokens, heads, dim = k.shape
     ks, vs = k.stride(), v.stride()
     if dim > 1 and (ks[2] != 1 or vs[2] != 1):
         _refuse(where, "the head dimension of k and v must be contiguous")
-    _check_ints(where, device, slots=slots)
+    _check_ints(where, index, slots=slots)
     if slots.numel() < tokens:
         _refuse(where, f"{slots.numel()} slots for {tokens} tokens")
     code, ksp, vsp = _check_cache(where, k_cache, v_cache, k.dtype, k_scale, v_scale)
     pages, page, cache_heads, cache_dim = k_cache.shape
-    if (cache_heads, cache_dim) != (heads, dim) or k_cache.device != device:
+    if (cache_heads, cache_dim) != (heads, dim) or k_cache.get_device() != index:
         _refuse(where, "the caches must be on the device of k and v and have their heads and dim")
-    if not k.is_cuda:
+    if index < 0:
         _refuse(where, "the tensors must be on a CUDA device")
     if tokens == 0:
         return
     cs = k_cache.stride()
-    index = device.index
     args = L.pack_paged_append(
         k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp,
-        _check_status(where, device, status), ks[0], ks[1], vs[0], vs[1], cs[0], cs[1], cs[2], tokens, heads, dim, page, pages,
+        _check_status(where, index, status), ks[0], ks[1], vs[0], vs[1], cs[0], cs[1], cs[2], tokens, heads, dim, page, pages,
         _DTYPES[k.dtype], code, index)
     rc = L.lib().syn_paged_append(args, _stream(index, stream))
     if rc:
         L.check(rc, "syn_paged_append")
 
 
-def _workspace(device: torch.device, num_sms: int, dim: int):
-    key = (device.index, num_sms, dim)
+def _workspace(device: torch.device, index: int, num_sms: int, dim: int):
+    key = (index, num_sms, dim)
     size = _WORKSPACE_BYTES.get(key)
     if size is None:
-        sms = num_sms or torch.cuda.get_device_properties(device).multi_processor_count
+        most = torch.cuda.get_device_properties(device).multi_processor_count
+        sms = min(num_sms or most, most)
         size = _WORKSPACE_BYTES[key] = L.lib().syn_paged_attention_workspace(sms, dim)
     # From torch's allocator at every call: calls on different streams and captured graphs never share it.
     return torch.empty(size, dtype=torch.uint8, device=device), size
@@ -247,19 +250,19 @@ def paged_attention(
         _refuse(where, "q must be an fp16/bf16 tensor")
     if q.dim() != 3:
         _refuse(where, "q must be [tokens, q_heads, dim]")
-    device = q.device
+    index = q.get_device()
     tokens, q_heads, dim = q.shape
     qs = q.stride()
     if qs[2] != 1 or dim not in HEAD_DIMS:
         _refuse(where, f"the head dimension must be contiguous and one of {HEAD_DIMS}")
     code, ksp, vsp = _check_cache(where, k_cache, v_cache, dtype, k_scale, v_scale)
     pages, page, heads, cache_dim = k_cache.shape
-    if cache_dim != dim or k_cache.device != device:
+    if cache_dim != dim or k_cache.get_device() != index:
         _refuse(where, "the caches must be on the device of q and have its head dimension")
     if heads == 0 or q_heads == 0 or q_heads % heads:
         _refuse(where, f"{q_heads} query heads over {heads} key-value heads")
-    table_stride = _check_table(where, device, table)
-    _check_ints(where, device, lens=lens)
+    table_stride = _check_table(where, index, table)
+    _check_ints(where, index, lens=lens)
     requests, width = table.shape
     if lens.numel() != requests:
         _refuse(where, "lens needs one entry a row of table")
@@ -267,39 +270,40 @@ def paged_attention(
         if tokens != requests:
             _refuse(where, f"{tokens} rows of q for {requests} requests: pass starts")
     else:
-        _check_ints(where, device, starts=starts)
+        _check_ints(where, index, starts=starts)
         if starts.numel() != requests + 1:
             _refuse(where, "starts needs one entry more than table has rows")
     if window < 0 or (window and not causal):
         _refuse(where, "window must not be negative and needs causal=True")
+    if num_sms < 0:
+        _refuse(where, "num_sms must not be negative")
     if out is not None:
-        if out.dtype is not dtype or out.shape != q.shape or out.device != device or out.stride(2) != 1:
+        if out.dtype is not dtype or out.shape != q.shape or out.get_device() != index or out.stride(2) != 1:
             _refuse(where, "out must have the shape, type and device of q and a contiguous head dimension")
         if out.data_ptr() == q.data_ptr() and tokens:
             _refuse(where, "out must not overlap q")
-    if lse is not None and (lse.dtype is not torch.float32 or lse.device != device or lse.shape != q.shape[:2]
+    if lse is not None and (lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != q.shape[:2]
                             or not lse.is_contiguous()):
         _refuse(where, "lse must be a contiguous float32 [tokens, q_heads] tensor on the device of q")
-    if not q.is_cuda:
+    if index < 0:
         _refuse(where, "the tensors must be on a CUDA device")
     if stream is not None:
-        _stream(device.index, stream)
-        # What is allocated below belongs to the stream that it is used on.
+        _stream(index, stream)
+        # What is allocated below belongs to the stream that it is used on, and to the device of that stream.
         with torch.cuda.stream(stream):
             return paged_attention(q, k_cache, v_cache, table, lens, sm_scale, starts=starts, causal=causal, window=window,
                                    k_scale=k_scale, v_scale=v_scale, out=out, lse=lse, num_sms=num_sms, status=status)
     if out is None:
-        out = (torch.empty if starts is None else torch.zeros)(tokens, q_heads, dim, dtype=dtype, device=device)
+        out = (torch.empty if starts is None else torch.zeros)(tokens, q_heads, dim, dtype=dtype, device=q.device)
     if tokens == 0 or requests == 0:
         return out
     os_ = out.stride()
     cs = k_cache.stride()
-    index = device.index
-    workspace, size = _workspace(device, num_sms, dim)
+    workspace, size = _workspace(q.device, index, num_sms, dim)
     args = L.pack_paged_attn(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),
         0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), ksp, vsp,
-        workspace.data_ptr(), size, _check_status(where, device, status), qs[0], qs[1],
+        workspace.data_ptr(), size, _check_status(where, index, status), qs[0], qs[1],
         os_[0], os_[1], cs[0], cs[1], cs[2], table_stride, sm_scale, tokens, requests, q_heads, heads, dim, page,
         pages, width, 1 if causal else 0, window, _DTYPES[dtype], code, num_sms, index)
     rc = L.lib().syn_paged_attention(args, _stream(index, None))

@@ -142,6 +142,7 @@ extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
   if (a->cache_dtype != SYN_CACHE_SAME && a->cache_dtype != SYN_CACHE_E4M3) return SYN_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a->num_pages) * a->page_size > INT_MAX) return SYN_ERR_TOO_LARGE;
   if (a->tokens == 0) return SYN_OK;
+  if (a->tokens > INT_MAX / 2 / (a->Hq / a->Hkv)) return SYN_ERR_TOO_LARGE;  // rows of a head
   syn_paged_attn_args p = *a;
   const bool e4m3 = a->cache_dtype == SYN_CACHE_E4M3;
   if (a->q == nullptr || a->k_cache == nullptr || a->v_cache == nullptr || a->table == nullptr || a->lens == nullptr ||
@@ -156,6 +157,8 @@ extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
     return SYN_ERR_INVALID;
   PagedDevice device(a->device);
   SYN_CUDA_TRY(device.error());
+  // So that positions less the window stay numbers of 32 bits.
+  if (p.window > INT_MAX - 64 - a->tokens) p.window = INT_MAX - 64 - a->tokens;
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != SYN_OK) return rc;

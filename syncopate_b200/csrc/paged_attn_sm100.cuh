@@ -191,9 +191,9 @@ __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args&
     r.s0 = min(max(a.starts[z], 0), a.tokens);
     r.n = min(max(a.starts[z + 1], r.s0), a.tokens) - r.s0;
   }
+  // One key too many stands for all that the table has no room for; 64 keeps key numbers from passing 2^31.
   const long long room = static_cast<long long>(a.width) * a.page_size;
-  int len = max(a.lens[z], 0);
-  if (len > room) len = static_cast<int>(min(room + 1, static_cast<long long>(INT_MAX)));
+  const int len = static_cast<int>(min(min(static_cast<long long>(max(a.lens[z], 0)), room + 1), static_cast<long long>(INT_MAX - 64)));
   r.len = len;
   r.first = a.window > 0 ? max(0, min(len, len - r.n - a.window + 1)) : 0;
   r.steps = max(1, (len - r.first + C::KEYS - 1) / C::KEYS);

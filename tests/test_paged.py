@@ -112,6 +112,7 @@ def _attend_tensors():
     (dict(starts=torch.zeros(3, **I32)), "starts needs"),
     (dict(window=-1), "window"),
     (dict(window=4, causal=False), "window"),
+    (dict(num_sms=-1), "num_sms"),
     (dict(out=torch.zeros(3, 4, 64, dtype=HF)), "out must have"),
     (dict(lse=torch.zeros(3, 4, dtype=BF)), "lse must be"),
     (dict(lse=torch.zeros(4, 3).t()), "lse must be"),

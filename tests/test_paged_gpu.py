@@ -310,6 +310,22 @@ def test_long_requests_are_split_and_joined(kept, num_sms):
     _check_attention([12345, 777], [3, 5], 14, 2, 64, 32, HF, E4 if kept is E4 else HF, num_sms=num_sms, window=5000)
 
 
+@pytest.mark.parametrize("dim, kept, heads", [(64, E4, 4), (64, E4, 8), (64, HF, 6), (128, E4, 4), (128, E4, 3), (256, E4, 2)])
+@pytest.mark.parametrize("num_sms", [0, 2])
+def test_heads_taken_side_by_side(dim, kept, heads, num_sms):
+    _check_attention(EDGES + [7001], None, 4 * heads, heads, dim, 16, HF, kept, num_sms=num_sms, poison=True)
+    _check_attention([3000, 1, 0, 501], [5, 1, 2, 11], 6 * heads, heads, dim, 32, HF, kept, num_sms=num_sms, window=2000)
+
+
+@pytest.mark.parametrize("page", [2, 5, 7, 31, 33, 4096])
+def test_page_sizes_of_every_kind(page):
+    _check_attention([1, page, page + 1, 3 * page - 1, 2000], None, 4, 2, 64, page, BF, BF, poison=True)
+
+
+def test_the_largest_window():
+    _check_attention([300, 5], [4, 9], 4, 2, 64, 16, BF, BF, window=2 ** 31 - 1)
+
+
 def test_many_requests():
     rng = random.Random(1)
     _check_attention([rng.randint(0, 90) for _ in range(2100)], None, 4, 1, 64, 16, BF, BF)
@@ -423,6 +439,30 @@ def test_same_results_at_every_call_on_any_stream():
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, first)
+
+
+def test_two_graphs_replayed_at_once():
+    lens = [4000, 700, 9000]
+    gen, table, values, caches, _ = _make(lens, 16, 2, 128, BF, BF, 6)
+    q = [_normal(gen, 3, 8, 128, dtype=BF).cuda() for _ in range(2)]
+    table_t, lens_t = ints(table), ints(lens)
+    want = [paged_attention(x, *caches, table_t, lens_t, 0.1) for x in q]
+    outs, graphs = [torch.zeros_like(x) for x in q], []
+    for x, out in zip(q, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(8):
+                paged_attention(x, *caches, table_t, lens_t, 0.1, out=out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
 # ------------------------------------------------------------------ a run of steps
