@@ -16,7 +16,7 @@
 //     equal shares for the warps of a grid that fills the GPU, whatever the lengths; loads run on across the
 //     borders of units.  Where a head is less than 256 bytes and the heads of a token lie side by side, two or
 //     four warps take neighbouring heads at the same keys (`tracks`): HBM answers 128 bytes here and there a
-//     sixth slower than 256.  A unit that a border cuts leaves partial results, which a second small kernel joins
+//     tenth slower than 256 side by side, 64 bytes a third.  A unit that a border cuts leaves partial results, which a second small kernel joins
 //     in a fixed order (the warps of a block that work on one and the same unit join theirs first): results do
 //     not depend on timing, there are no atomics and no state between calls.
 #pragma once
@@ -33,7 +33,7 @@ constexpr int PA_THREADS = PA_WARPS * 32;
 // The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
 // than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
 constexpr float PA_SLACK = 8.f;
-constexpr float PA_NONE = -1e30f;
+constexpr float PA_NONE = -1e30f;  // reference of a row without a key so far
 constexpr int PA_DESC = 12;  // int32 words a worker leaves for the join (PagedJoin)
 
 struct PagedAttnParams {
@@ -80,7 +80,11 @@ struct PagedCfg {
   static constexpr int ROWB = D * (E4M3 ? 1 : 2);    // bytes of a stored head
   static constexpr int CPR = ROWB / 16;              // 16-byte chunks of it
   static constexpr int HALFB = KEYS * ROWB;          // the keys of a step, or its values
-  static constexpr int BLOCKS = D == 256 ? 3 - RT : RT == 1 || (RT == 2 && D == 64) ? 3 : 2;  // resident on an SM
+  // Blocks on an SM and halves in a ring: as many bytes on the way as shared memory holds, and the registers that the
+  // output leaves.  8 rows: three blocks of four slots; with four of three too little is on the way (2500-token
+  // requests 126 us against 115).  16 rows: two blocks where three leave too few registers (D = 128: 117 against
+  // 136), three where they do not (D = 64: 79 against 102).
+  static constexpr int BLOCKS = D == 256 ? 3 - RT : RT == 1 || (RT == 2 && D == 64) ? 3 : 2;
   static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? (RT == 1 ? 4 : 5) : (RT <= 2 ? 8 : 10);
   static constexpr int RING = SLOTS * HALFB;         // bytes a warp
   static constexpr bool QREG = RT * D <= 256;        // query fragments in registers, else in shared memory
@@ -479,8 +483,11 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   const long long t1 = works ? cut.at(worker + 1) : total;
   PagedJoin join;
   join.n1 = join.n2 = join.n3 = 0;
+  auto nothing_to_join = [&]() {
+    for (int i = 0; i < 2; ++i) reinterpret_cast<int4*>(record)[i] = make_int4(0, 0, 0, 0);  // the counts are in these
+  };
   if (t0 >= t1) {
-    if (lane == 0) *reinterpret_cast<int4*>(record) = make_int4(0, 0, 0, 0), reinterpret_cast<int4*>(record)[1] = make_int4(0, 0, 0, 0);
+    if (lane == 0) nothing_to_join();
     return;
   }
 
@@ -514,7 +521,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   }
   if (lane == 0) {
     if (join.parts() > 0) *reinterpret_cast<PagedJoin*>(record) = join;
-    else *reinterpret_cast<int4*>(record) = make_int4(0, 0, 0, 0), reinterpret_cast<int4*>(record)[1] = make_int4(0, 0, 0, 0);
+    else nothing_to_join();
   }
 
   // ---- producer: halves of steps (keys, values, keys, ...) are asked for SLOTS - 1 halves ahead, across units
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
         const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
         up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        const float back = mult * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+        const float back = copysignf(fmaxf(fabsf(mult) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), 1e-37f), mult);
 #pragma unroll
         for (int c = 0; c < 2; ++c) down[2 * i + c] = __shfl_sync(~0u, back, (2 * t4 + c) * 4);
       }
@@ -992,19 +999,19 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   }
 }
 
-// Joins the parts of the units that borders between workers cut.  Of a unit of few parts a warp takes four fragments
-// of the output; of one of many (a long request has hundreds) a block takes a fragment, and its warps share the
+// Joins the parts of the units that borders between workers cut.  Of a unit of few parts a warp takes up to eight
+// fragments of the output; of one of many (a long request has hundreds) a block takes a fragment, and its warps share the
 // parts.  The kernel runs for a few microseconds, most of which its first pass through its own code takes: the
 // loops stay rolled up (unrolled by 4 over parts and by 8 over fragments it took 24 us on 1776 units of two parts).
 constexpr int PA_JOIN_WARPS = 16;
 constexpr int PA_JOIN_MANY = 12;    // parts from which on a unit counts as one of many
-constexpr int PA_JOIN_FRAGS = 4;    // fragments a warp, of one 8-row tile
 constexpr int PA_JOIN_LOOK = 128;   // records that a block looks through for units of many parts
 
 // Blocks of the join: those for units of few parts, then those for units of many.
 template <typename C>
 struct PagedJoinGrid {
-  static constexpr int SLICES = C::FRAGS / PA_JOIN_FRAGS;
+  static constexpr int N = C::DT < 8 ? C::DT : 8;  // fragments a warp, of one 8-row tile
+  static constexpr int SLICES = C::FRAGS / N;
   int few, many;
   __host__ __device__ explicit PagedJoinGrid(int records)
       : few((records + PA_JOIN_WARPS - 1) / PA_JOIN_WARPS * SLICES), many((records + PA_JOIN_LOOK - 1) / PA_JOIN_LOOK * C::FRAGS) {}
@@ -1040,15 +1047,16 @@ __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __
   const PagedJoin* record = reinterpret_cast<const PagedJoin*>(p.desc);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < grid.few) {
+    constexpr int N = PagedJoinGrid<C>::N;
     const int slice = blockIdx.x % PagedJoinGrid<C>::SLICES, c = blockIdx.x / PagedJoinGrid<C>::SLICES * PA_JOIN_WARPS + warp;
-    const int j = slice % RT, dt = slice / RT * PA_JOIN_FRAGS;
+    const int j = slice % RT, dt = slice / RT * N;
     if (c >= records) return;
     const PagedJoin d = record[c];
     if (d.parts() == 0 || d.parts() >= PA_JOIN_MANY || j * 8 >= d.rows) return;
-    PagedSum<PA_JOIN_FRAGS> sum;
+    PagedSum<N> sum;
     sum.clear();
-    paged_merge<C, PA_JOIN_FRAGS, 2>(p, d, sum, dt, j, 0, 1, lane);
-    paged_finish<C, PA_JOIN_FRAGS>(p.a, sum.o, sum.m, sum.l, dt, d.s0, d.kv_head, d.row0 + j * 8, d.rows - j * 8, lane);
+    paged_merge<C, N, 2>(p, d, sum, dt, j, 0, 1, lane);
+    paged_finish<C, N>(p.a, sum.o, sum.m, sum.l, dt, d.s0, d.kv_head, d.row0 + j * 8, d.rows - j * 8, lane);
     return;
   }
   __shared__ float4 s_ml[PA_JOIN_WARPS][32], s_o[PA_JOIN_WARPS][32];
