@@ -1004,8 +1004,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 // parts.  The kernel runs for a few microseconds, most of which its first pass through its own code takes: the
 // loops stay rolled up (unrolled by 4 over parts and by 8 over fragments it took 24 us on 1776 units of two parts).
 constexpr int PA_JOIN_WARPS = 16;
-constexpr int PA_JOIN_MANY = 12;    // parts from which on a unit counts as one of many
-constexpr int PA_JOIN_LOOK = 128;   // records that a block looks through for units of many parts
+constexpr int PA_JOIN_MANY = 16;    // parts from which on a unit counts as one of many
+constexpr int PA_JOIN_LOOK = 32;    // records that a block looks through for units of many parts, which it takes one by
+                                    // one (16 requests, 8-bit, D = 64, 14 parts a unit: 71 us with 128 and 12, 49 so)
 
 // Blocks of the join: those for units of few parts, then those for units of many.
 template <typename C>
@@ -1060,20 +1061,15 @@ __global__ void __launch_bounds__(PA_JOIN_WARPS * 32) paged_join_kernel(const __
     return;
   }
   __shared__ float4 s_ml[PA_JOIN_WARPS][32], s_o[PA_JOIN_WARPS][32];
-  __shared__ uint32_t s_many[PA_JOIN_LOOK / 32];
   const int index = blockIdx.x - grid.few, f = index % C::FRAGS, c0 = index / C::FRAGS * PA_JOIN_LOOK;
   const int j = f % RT, dt = f / RT;
+  static_assert(PA_JOIN_LOOK == 32, "every warp looks for itself");
   int parts = 0;
-  if (threadIdx.x < PA_JOIN_LOOK && c0 + static_cast<int>(threadIdx.x) < records) parts = record[c0 + threadIdx.x].parts();
-  const uint32_t many = __ballot_sync(~0u, parts >= PA_JOIN_MANY);
-  if (lane == 0 && warp < PA_JOIN_LOOK / 32) s_many[warp] = many;
-  if (!__syncthreads_or(parts >= PA_JOIN_MANY)) return;
-  uint32_t left = s_many[0];
+  if (c0 + lane < records) parts = record[c0 + lane].parts();
+  uint32_t left = __ballot_sync(~0u, parts >= PA_JOIN_MANY);
 #pragma unroll 1
-  for (int group = 0;;) {
-    while (left == 0 && ++group < PA_JOIN_LOOK / 32) left = s_many[group];
-    if (left == 0) return;
-    const PagedJoin d = record[c0 + group * 32 + __ffs(left) - 1];
+  while (left != 0) {  // the same for all warps
+    const PagedJoin d = record[c0 + __ffs(left) - 1];
     left &= left - 1;
     if (j * 8 >= d.rows) continue;
     PagedSum<1> sum;
