@@ -465,6 +465,35 @@ def test_two_graphs_replayed_at_once():
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
+def test_rows_behind_the_last_request_without_an_output_given():
+    lens, starts = [30, 40], [0, 2, 3]
+    gen, table, values, caches, _ = _make(lens, 16, 2, 64, HF, HF, 8)
+    q = _normal(gen, 6, 4, 64, dtype=HF)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    args = (q.cuda(), *caches, ints(table), ints(lens), 0.1)
+    here = paged_attention(*args, starts=ints(starts))
+    torch.cuda.synchronize()
+    there = paged_attention(*args, starts=ints(starts), stream=stream)
+    torch.cuda.synchronize()
+    assert (here[3:] == 0).all() and torch.equal(here, there)
+    want = R.attention(q, values[0], values[1], table, lens, 0.1, starts)
+    _compare(here[:3].cpu(), want[1][:3].float(), [w[:3] for w in want])
+    with pytest.raises(ValueError, match="8-bit"):
+        paged_attention(*args, starts=ints(starts), k_scale=torch.ones(2, device="cuda"), v_scale=torch.ones(2, device="cuda"))
+
+
+def test_scores_that_all_vanish_over_an_8_bit_cache():
+    # A scale of zero and queries next to nothing: every key counts alike.
+    gen, table, values, caches, scales = _make([37, 50], 16, 2, 128, BF, E4, 12)
+    q = (_normal(gen, 5, 8, 128) * 1e-25).to(BF)
+    for sm_scale in (0.0, 1.0):
+        lse = torch.empty(5, 8, device="cuda")
+        out = paged_attention(q.cuda(), *caches, ints(table), ints([37, 50]), sm_scale, starts=ints([0, 3, 5]), window=20,
+                              k_scale=scales[0].cuda(), v_scale=scales[1].cuda(), lse=lse)
+        _compare(out.cpu(), lse.cpu(), R.attention(q, values[0], values[1], table, [37, 50], sm_scale, [0, 3, 5], True, 20, *scales))
+
+
 # ------------------------------------------------------------------ a run of steps
 def _drive(cache, steps, q_heads, heads, dim, dtype, graph):
     """Random steps over the cache object; the same tokens are kept densely on the side."""
@@ -550,7 +579,7 @@ def _drive(cache, steps, q_heads, heads, dim, dtype, graph):
 def test_a_run_of_steps(graph, kept):
     heads, q_heads, dim, layers = 2, 8, 128, 2
     scales = {} if kept is None else dict(k_scale=torch.rand(layers, heads) * 0.01 + 0.01, v_scale=torch.rand(layers, heads) * 0.01 + 0.01)
-    cache = PagedKVCache(200, 8, heads, dim, 9, 150, 64, layers=layers, dtype=BF, cache_dtype=kept, **scales)
+    cache = PagedKVCache(200, 8, heads, dim, 9, 150, 64, layers=layers, dtype=BF, cache_dtype=kept, device="cuda:0", **scales)
     cache.kv.view(torch.uint8).fill_(0xFF)  # NaN in every slot that nothing was written to
     _drive(cache, 25, q_heads, heads, dim, BF, graph)
 
