@@ -25,6 +25,8 @@ NVCC_FLAGS = [
     "-Xcompiler",
     "-fPIC",
     "-shared",
+    "--threads",  # one compilation a core
+    "0",
 ]
 
 
