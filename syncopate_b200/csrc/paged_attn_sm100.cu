@@ -164,6 +164,8 @@ extern "C" int syn_paged_attention(const syn_paged_attn_args* a, void* stream) {
   SYN_CUDA_TRY(device.error());
   // So that positions less the window stay numbers of 32 bits.
   if (p.window > INT_MAX - 64 - a->tokens) p.window = INT_MAX - 64 - a->tokens;
+  // So that numbers of keys do: what lies behind counts as behind the table.
+  if (p.width > (INT_MAX - 64) / a->page_size) p.width = (INT_MAX - 64) / a->page_size;
   int sms = 0;
   const int rc = device_sm_count(&sms);
   if (rc != SYN_OK) return rc;

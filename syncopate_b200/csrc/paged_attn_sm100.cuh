@@ -183,9 +183,16 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 struct PagedRequest {
   int s0, n;       // rows of q: first one, how many
   int len;         // keys (one more than the table has room for, where the length says more)
+  int pos0;        // position of the first row, by the length as it is given (rows behind the table stay behind it)
   int first;       // first key that any row sees
   int steps, rt;   // steps of a unit; row tiles a head
 };
+
+// First key that the window leaves to position `at`; the key that stands for those behind the table is left to every
+// position behind it, which so becomes NaN.
+__device__ __forceinline__ int paged_window_from(const syn_paged_attn_args& a, const PagedRequest& r, int at) {
+  return min(at - a.window + 1, r.len - 1);
+}
 
 template <typename C>
 __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args& a, int z) {
@@ -195,12 +202,12 @@ __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args&
     r.s0 = min(max(a.starts[z], 0), a.tokens);
     r.n = min(max(a.starts[z + 1], r.s0), a.tokens) - r.s0;
   }
-  // One key too many stands for all that the table has no room for; 64 keeps key numbers from passing 2^31.
-  const long long room = static_cast<long long>(a.width) * a.page_size;
-  const int len = static_cast<int>(min(min(static_cast<long long>(max(a.lens[z], 0)), room + 1), static_cast<long long>(INT_MAX - 64)));
-  r.len = len;
-  r.first = a.window > 0 ? max(0, min(len, len - r.n - a.window + 1)) : 0;
-  r.steps = max(1, (len - r.first + C::KEYS - 1) / C::KEYS);
+  // One key too many stands for all that the table has no room for (the host keeps the room below 2^31 - 64).
+  const int room = a.width * a.page_size, len = max(a.lens[z], 0);
+  r.len = min(len, room + 1);
+  r.pos0 = len - r.n;
+  r.first = a.window > 0 ? max(0, paged_window_from(a, r, r.pos0)) : 0;
+  r.steps = max(1, (r.len - r.first + C::KEYS - 1) / C::KEYS);
   r.rt = (r.n * (a.Hq / a.Hkv) + C::ROWS - 1) / C::ROWS;
   return r;
 }
@@ -617,7 +624,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const PagedRequest r = cur.r;
     const int head_group = cur.sub / r.rt, kv_head = head_group * p.tracks + track, row0 = (cur.sub - head_group * r.rt) * C::ROWS;
     const int rows = min(C::ROWS, r.n * group - row0);
-    const int pos0 = r.len - r.n;
+    const int pos0 = r.pos0;
     const bool one = r.n == 1;  // one new token: spares the divisions
     const int steps = static_cast<int>(min(static_cast<long long>(r.steps - cur.step), t1 - t));
     // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
@@ -629,7 +636,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       pos[x] = pos0 + tok;
     }
     // Keys lo .. hi - 1 are seen from position `at`.
-    auto lo = [&](int at) { return a.window > 0 ? at - a.window + 1 : 0; };
+    auto lo = [&](int at) { return a.window > 0 ? paged_window_from(a, r, at) : 0; };
     auto hi = [&](int at) { return a.causal ? min(r.len, at + 1) : r.len; };
     // From product to power of two; a key that is not seen gets the product that stands for a power of -inf, so the
     // factor must not be 0 (which 1e-30 stands for: scores then differ by less than a rounding).

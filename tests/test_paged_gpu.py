@@ -604,3 +604,27 @@ def test_a_step_that_does_not_fit_is_told_and_changes_nothing():
     cache.plan(ints([-1, 16]))  # the first request makes room
     cache.check()
     assert cache.lens.tolist() == [0, 17] and cache.num_free.tolist() == [1]
+
+
+@pytest.mark.parametrize("kept", [BF, E4])
+@pytest.mark.parametrize("window", [0, 1, 7, 40, 200])
+@pytest.mark.parametrize("past", [1, 3, 5, 9, 60, 2 ** 31 - 1 - 112])
+def test_new_tokens_behind_the_row_of_the_table(kept, window, past):
+    """Request 0 says that it is `past` tokens longer than its row of the table has room for: its tokens from there on
+    need a key that no page holds, those before are where they say they are."""
+    page, room, news, heads, q_heads, dim = 16, 112, [5, 3], 2, 8, 128
+    gen, table, values, caches, scales = _make([room, 50], page, heads, dim, BF, kept, 31)
+    q = _normal(gen, 8, q_heads, dim, dtype=BF)
+    there = max(0, news[0] - past)  # tokens before the end of the table
+    rows = list(range(there)) + [5, 6, 7]
+    for causal in (True, False) if window == 0 else (True,):
+        status, lse = ints([0] * 4), torch.empty(8, q_heads, device="cuda")
+        out = paged_attention(q.cuda(), *caches, ints(table), ints([room + past, 50]), 0.1, starts=ints([0, 5, 8]), causal=causal,
+                              window=window, k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse, status=status).cpu()
+        assert status.tolist()[:2] == [5, 0]
+        seen = rows if causal else rows[there:]
+        gone = [i for i in range(8) if i not in seen]
+        assert torch.isnan(out[gone].float()).all() and torch.isnan(lse.cpu()[gone]).all()
+        want = R.attention(q[rows], values[0], values[1], table, [room, 50], 0.1, [0, there, there + 3], causal, window, *scales)
+        at = [rows.index(i) for i in seen]
+        _compare(out[seen], lse.cpu()[seen], [w[at] for w in want])
