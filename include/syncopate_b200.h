@@ -536,9 +536,9 @@ int syn_paged_append(const syn_paged_append_args* args, void* stream);
  *   o = sum_j softmax_j(q . k_j * sm_scale) v_j,  lse [tokens, Hq] (may be NULL) = log2 sum_j exp(...)
  * Keys and values of an 8-bit cache count as k_scale[head] and v_scale[head] times what is stored.  A row
  * that sees no key gives 0 and lse = -inf; keys and values that a row does not see do not touch it,
- * whatever they hold.  Rows outside all requests are left as they were.  A row that should see a key
- * behind its row of the table (or from key 2^31 - 64 - page_size on), or on a page outside [0, num_pages), comes out as
- * NaN (and in `status`).
+ * whatever they hold.  Rows outside all requests are left as they were.  A request with rows behind the end of q is
+ * told in `status`; its rows before the end stay in their places.  A row that should see a key behind its row of the
+ * table (or from key 2^31 - 64 - page_size on), or on a page outside [0, num_pages), comes out as NaN (and in `status`).
  * Base addresses and strides (in bytes) are multiples of 16.
  * `workspace`: syn_paged_attention_workspace bytes, 16-byte aligned, any contents; it belongs to the call
  * until the call has ended on the GPU. */

@@ -183,7 +183,8 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 struct PagedRequest {
   int s0, n;       // rows of q: first one, how many
   int len;         // keys (one more than the table has room for, where the length says more)
-  int pos0;        // position of the first row, by the length as it is given (rows behind the table stay behind it)
+  int pos0;        // position of the first row, by length and border as they are given: rows behind the table stay
+                   // behind it, and rows that q does not have do not move those that it has
   int first;       // first key that any row sees
   int steps, rt;   // steps of a unit; row tiles a head
 };
@@ -198,14 +199,16 @@ template <typename C>
 __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args& a, int z) {
   PagedRequest r;
   r.s0 = z, r.n = 1;
+  int end = z + 1;  // behind the request's last row
   if (a.starts != nullptr) {
     r.s0 = min(max(a.starts[z], 0), a.tokens);
-    r.n = min(max(a.starts[z + 1], r.s0), a.tokens) - r.s0;
+    end = max(a.starts[z + 1], r.s0);
+    r.n = min(end, a.tokens) - r.s0;
   }
   // One key too many stands for all that the table has no room for (the host keeps the room below 2^31 - 64).
   const int room = a.width * a.page_size, len = max(a.lens[z], 0);
   r.len = min(len, room + 1);
-  r.pos0 = len - r.n;
+  r.pos0 = max(len - (end - r.s0), -a.tokens);  // (a row at a position below 0 sees nothing)
   r.first = a.window > 0 ? max(0, paged_window_from(a, r, r.pos0)) : 0;
   r.steps = max(1, (r.len - r.first + C::KEYS - 1) / C::KEYS);
   r.rt = (r.n * (a.Hq / a.Hkv) + C::ROWS - 1) / C::ROWS;

@@ -628,3 +628,18 @@ def test_new_tokens_behind_the_row_of_the_table(kept, window, past):
         want = R.attention(q[rows], values[0], values[1], table, [room, 50], 0.1, [0, there, there + 3], causal, window, *scales)
         at = [rows.index(i) for i in seen]
         _compare(out[seen], lse.cpu()[seen], [w[at] for w in want])
+
+
+@pytest.mark.parametrize("kept", [BF, E4])
+@pytest.mark.parametrize("window, causal", [(0, True), (0, False), (1, True), (9, True)])
+def test_fewer_rows_than_the_requests_say(kept, window, causal):
+    # Request 1 has two of its five rows behind the end of q, request 2 all of them: the rows that are there stay in place.
+    lens, starts, heads, q_heads, dim = [40, 70, 33], [0, 4, 9, 11], 2, 8, 128
+    gen, table, values, caches, scales = _make(lens, 16, heads, dim, BF, kept, 32)
+    q = _normal(gen, 11, q_heads, dim, dtype=BF)
+    want = R.attention(q, values[0], values[1], table, lens, 0.1, starts, causal, window, *scales)
+    status, lse = ints([0] * 4), torch.empty(7, q_heads, device="cuda")
+    out = paged_attention(q[:7].cuda(), *caches, ints(table), ints(lens), 0.1, starts=ints(starts), causal=causal, window=window,
+                          k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse, status=status)
+    assert status.tolist()[0] == 5
+    _compare(out.cpu(), lse.cpu(), [w[:7] for w in want])
