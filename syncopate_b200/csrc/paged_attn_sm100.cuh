@@ -146,6 +146,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
+// TF32: numbers of 32 bits whose lower 13 are 0.
+__device__ __forceinline__ void mma1688_tf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
+        "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -191,8 +199,8 @@ struct PagedRequest {
 
 // First key that the window leaves to position `at`; the key that stands for those behind the table is left to every
 // position behind it, which so becomes NaN.
-__device__ __forceinline__ int paged_window_from(const syn_paged_attn_args& a, const PagedRequest& r, int at) {
-  return min(at - a.window + 1, r.len - 1);
+__device__ __forceinline__ int paged_window_from(const syn_paged_attn_args& a, int len, int at) {
+  return min(at - a.window + 1, len - 1);
 }
 
 template <typename C>
@@ -209,7 +217,7 @@ __device__ __forceinline__ PagedRequest paged_request(const syn_paged_attn_args&
   const int room = a.width * a.page_size, len = max(a.lens[z], 0);
   r.len = min(len, room + 1);
   r.pos0 = max(len - (end - r.s0), -a.tokens);  // (a row at a position below 0 sees nothing)
-  r.first = a.window > 0 ? max(0, paged_window_from(a, r, r.pos0)) : 0;
+  r.first = a.window > 0 ? max(0, paged_window_from(a, r.len, r.pos0)) : 0;
   r.steps = max(1, (r.len - r.first + C::KEYS - 1) / C::KEYS);
   r.rt = (r.n * (a.Hq / a.Hkv) + C::ROWS - 1) / C::ROWS;
   return r;
@@ -304,6 +312,125 @@ __device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
         words(half * 8 + 4, x0.z, x1.z, x8.z, x9.z);
         words(half * 8 + 6, x0.w, x1.w, x8.w, x9.w);
       }
+    }
+  }
+}
+
+// The weights of an 8-row tile at 16 keys, from the scores' fragment (keys by rows) to the values' products: each as two
+// numbers of fewer bits, the second one what the first left, so that their rounding does not add to that of the output.
+// bf16 values: two bf16 (16 bits).  Halves, 8-bit values among them: two TF32 (20 bits).  Two halves would be twice as fast
+// a product but lose the weights 2^-14 and more below the largest, and where a key takes the weight and its values are
+// small the output is made of those.  What it costs: nothing with 8 rows of 128 16-bit dimensions (113 us), 8-bit caches
+// 0.5 % (D = 64: 70 us -> 77), 32 rows 437 us -> 524 (8 bits 413 -> 468).
+template <bool BF16>
+struct PagedWeights;
+
+template <>
+struct PagedWeights<true> {
+  uint32_t hi[2], lo[2];
+  __device__ __forceinline__ void set(const float (&w)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t top = pack2<true>(w[2 * h], w[2 * h + 1]);
+      hi[h] = transpose8(top);
+      const float2 b = unpack2<true>(top);
+      lo[h] = transpose8(pack2<true>(w[2 * h] - b.x, w[2 * h + 1] - b.y));
+    }
+  }
+};
+
+template <>
+struct PagedWeights<false> {
+  float hi[2][2], lo[2][2];  // [8 keys each][key 2 t4, 2 t4 + 1] of row g
+  __device__ __forceinline__ void set(const float (&w)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t x = __float_as_uint(w[2 * h]), y = __float_as_uint(w[2 * h + 1]);
+      const uint32_t top = transpose8(__byte_perm(x, y, 0x7632)), low = transpose8(__byte_perm(x, y, 0x5410));
+      const uint32_t z[2] = {__byte_perm(low, top, 0x5410), __byte_perm(low, top, 0x7632)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        hi[h][i] = __uint_as_float(z[i] & 0xFFFFE000u);
+        lo[h][i] = __uint_as_float(__float_as_uint(__uint_as_float(z[i]) - hi[h][i]) & 0xFFFFE000u);
+      }
+    }
+  }
+};
+
+// A fragment of the values (16 dimensions by 16 keys) and its product with weights.
+template <bool BF16>
+struct PagedValues;
+
+template <>
+struct PagedValues<true> {
+  const uint32_t (&v)[4];
+  __device__ __forceinline__ explicit PagedValues(const uint32_t (&v_)[4]) : v(v_) {}
+  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<true>& w) const {
+    mma16816<true>(c, v, w.hi[0], w.hi[1]);
+    mma16816<true>(c, v, w.lo[0], w.lo[1]);
+  }
+};
+
+template <>
+struct PagedValues<false> {
+  float v[2][4];  // of 8 keys each: the even keys of dimensions g and g + 8, the odd ones (an order that the weights share)
+  __device__ __forceinline__ explicit PagedValues(const uint32_t (&u)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 x = unpack2<false>(u[2 * h]), y = unpack2<false>(u[2 * h + 1]);
+      v[h][0] = x.x, v[h][1] = y.x, v[h][2] = x.y, v[h][3] = y.y;
+    }
+  }
+  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<false>& w) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mma1688_tf32(c, v[h], w.hi[h][0], w.hi[h][1]);
+      mma1688_tf32(c, v[h], w.lo[h][0], w.lo[h][1]);
+    }
+  }
+};
+
+// Keys from .. to - 1 are seen from position `at` of a request.
+__device__ __forceinline__ int paged_seen_from(const syn_paged_attn_args& a, int len, int at) {
+  return a.window > 0 ? paged_window_from(a, len, at) : 0;
+}
+__device__ __forceinline__ int paged_seen_to(const syn_paged_attn_args& a, int len, int at) {
+  return a.causal ? min(len, at + 1) : len;
+}
+
+// Values that are not finite, at keys that only some rows see.  Zero times infinity: they may only enter the rows that see
+// them, so these groups of 16 keys (set in `groups`, the step's first key is `base`) are taken one row at a time, with what
+// it does not see taken out.  A function of its own, whose operands go through memory: inlined, its registers cost the steps
+// without such values (32 rows, 8-bit cache: 624 us against 468).
+template <typename C>
+struct alignas(16) PagedOdd {
+  float o[C::DT][C::RT][4], w[C::KEYS / 16][C::RT][4];
+  int pos[2 * C::RT];
+};
+template <typename C>
+__device__ __noinline__ void paged_odd(PagedOdd<C>& x, uint32_t v_at, int base, uint32_t groups, const syn_paged_attn_args& a, int len) {
+  constexpr bool MBF16 = std::is_same<typename C::type, __nv_bfloat16>::value && !C::E4M3;
+  const int lane = threadIdx.x & 31, t4 = lane & 3;
+#pragma unroll 1
+  for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+    if ((groups >> kk & 1) == 0) continue;
+#pragma unroll 1
+    for (int row = 0; row < C::ROWS; ++row) {  // column row % 2 of the lanes with t4 == row % 8 / 2
+      const int j = row >> 3, at = __shfl_sync(~0u, x.pos[2 * j + (row & 1)], row >> 1 & 3);
+      const int from = paged_seen_from(a, len, at), to = paged_seen_to(a, len, at), key = base + kk * 16 + t4 * 2;
+      auto seen = [&](int k) { return (k >= from && k < to ? 0xFFFFu : 0u) | (k + 1 >= from && k + 1 < to ? 0xFFFF0000u : 0u); };
+      const uint32_t mask0 = seen(key), mask1 = seen(key + 8);
+      PagedWeights<MBF16> w;
+      w.set(x.w[kk][j]);
+      each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
+        const uint32_t u[4] = {v[0] & mask0, v[1] & mask0, v[2] & mask1, v[3] & mask1};
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        PagedValues<MBF16>(u).times(c, w);
+        if (t4 == (row >> 1 & 3)) {
+          x.o[dt][j][row & 1] += row & 1 ? c[1] : c[0];
+          x.o[dt][j][2 + (row & 1)] += row & 1 ? c[3] : c[2];
+        }
+      });
     }
   }
 }
@@ -638,9 +765,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       const int tok = one ? 0 : (row0 + min((x >> 1) * 8 + 2 * t4 + (x & 1), rows - 1)) / group;
       pos[x] = pos0 + tok;
     }
-    // Keys lo .. hi - 1 are seen from position `at`.
-    auto lo = [&](int at) { return a.window > 0 ? paged_window_from(a, r, at) : 0; };
-    auto hi = [&](int at) { return a.causal ? min(r.len, at + 1) : r.len; };
+    auto lo = [&](int at) { return paged_seen_from(a, r.len, at); };
+    auto hi = [&](int at) { return paged_seen_to(a, r.len, at); };
     // From product to power of two; a key that is not seen gets the product that stands for a power of -inf, so the
     // factor must not be 0 (which 1e-30 stands for: scores then differ by less than a rounding).
     float mult = a.sm_scale * CUDART_L2E_F;
@@ -867,65 +993,52 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       const uint32_t v_at = ready();
       refill(true);
 
-      // ---- values, transposed: 16 dimensions by 8 rows a product.  The weights enter as two 16-bit numbers, the
-      // second one what the first left, so that their rounding does not add to that of the output.
+      // ---- values, transposed: 16 dimensions by 8 rows a product
+      uint32_t odd = 0;  // groups of 16 keys with values that are not finite, where not every row sees every key
+      if (!whole && r.n > 1) {
+        constexpr uint32_t EXP = MBF16 ? 0x7F807F80u : 0x7C007C00u, ONE = MBF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
-      for (int kk = 0; kk < SN; ++kk) {
-        uint32_t ph[RT][2], pl[RT][2];
+        for (int kk = 0; kk < SN; ++kk) {
+          bool any = false;
+          each_v<C>(v_at, lane, kk, [&](int, const uint32_t (&v)[4]) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) any |= (((v[c] & EXP) + ONE) & 0x80008000u) != 0;
+          });
+          if (__any_sync(~0u, any)) odd |= 1u << kk;
+        }
+      }
+      if (odd != 0) {
+        PagedOdd<C> x;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+          x.pos[2 * j] = pos[2 * j], x.pos[2 * j + 1] = pos[2 * j + 1];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int dt = 0; dt < C::DT; ++dt) x.o[dt][j][c] = o[dt][j][c];
+#pragma unroll
+            for (int n = 0; n < SN; ++n) x.w[n][j][c] = s[n][j][c];
+          }
+        }
+        paged_odd<C>(x, v_at, base, odd, a, r.len);
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float w0 = s[kk][j][2 * h], w1 = s[kk][j][2 * h + 1];
-            const uint32_t top = pack2<MBF16>(w0, w1);
-            ph[j][h] = transpose8(top);
-            const float2 b = unpack2<MBF16>(top);
-            pl[j][h] = transpose8(pack2<MBF16>(w0 - b.x, w1 - b.y));
-          }
-        bool odd = false;  // values that are not finite, at keys that not every row sees
-        if (!whole && r.n > 1) {
-          constexpr uint32_t EXP = MBF16 ? 0x7F807F80u : 0x7C007C00u, ONE = MBF16 ? 0x00800080u : 0x04000400u;
-          each_v<C>(v_at, lane, kk, [&](int, const uint32_t (&v)[4]) {
+          for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) odd |= (((v[c] & EXP) + ONE) & 0x80008000u) != 0;
-          });
-          odd = __any_sync(~0u, odd);
-        }
-        if (!odd) {
-          each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
+            for (int c = 0; c < 4; ++c) o[dt][j][c] = x.o[dt][j][c];
+      }
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-              mma16816<MBF16>(o[dt][j], v, ph[j][0], ph[j][1]);
-              mma16816<MBF16>(o[dt][j], v, pl[j][0], pl[j][1]);
-            }
-          });
-        } else {
-          // Zero times infinity: such values may only enter the rows that see them, so one row at a time,
-          // with what it does not see taken out.
+      for (int kk = 0; kk < SN; ++kk) {
+        if ((odd >> kk & 1) != 0) continue;
+        PagedWeights<MBF16> w[RT];
 #pragma unroll
-          for (int x = 0; x < 2 * RT; ++x) {
-            const int j = x >> 1;
-#pragma unroll 1
-            for (int q = 0; q < 4; ++q) {  // row 8 j + 2 q + (x & 1), a column of lanes t4 == q
-              const int at = __shfl_sync(~0u, pos[x], q), row_lo = lo(at), row_hi = hi(at);
-              const int key = base + kk * 16 + t4 * 2;
-              auto seen = [&](int k) {
-                return (k >= row_lo && k < row_hi ? 0xFFFFu : 0u) | (k + 1 >= row_lo && k + 1 < row_hi ? 0xFFFF0000u : 0u);
-              };
-              const uint32_t mask0 = seen(key), mask1 = seen(key + 8);
-              each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
-                const uint32_t u[4] = {v[0] & mask0, v[1] & mask0, v[2] & mask1, v[3] & mask1};
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<MBF16>(c, u, ph[j][0], ph[j][1]);
-                mma16816<MBF16>(c, u, pl[j][0], pl[j][1]);
-                if (t4 == q) {
-                  o[dt][j][x & 1] += c[x & 1];
-                  o[dt][j][2 + (x & 1)] += c[2 + (x & 1)];
-                }
-              });
-            }
-          }
-        }
+        for (int j = 0; j < RT; ++j) w[j].set(s[kk][j]);
+        each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
+          const PagedValues<MBF16> x(v);
+#pragma unroll
+          for (int j = 0; j < RT; ++j) x.times(o[dt][j], w[j]);
+        });
       }
     }
 

@@ -643,3 +643,55 @@ def test_fewer_rows_than_the_requests_say(kept, window, causal):
                           k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse, status=status)
     assert status.tolist()[0] == 5
     _compare(out.cpu(), lse.cpu(), [w[:7] for w in want])
+
+
+# (bits below the first key, the same a little lower), both of them numbers of the 8-bit type
+DEPTHS = [(8, 9), (14, 15), (18, 20), (22, 24), (26, 28), (40, 44), (72, 80)]
+
+
+@pytest.mark.parametrize("dtype, kept", [(BF, BF), (HF, HF), (BF, E4), (HF, E4)])
+@pytest.mark.parametrize("dim, group", [(64, 4), (64, 40), (128, 8), (128, 16), (128, 32), (256, 8), (256, 16)])
+@pytest.mark.parametrize("depth", DEPTHS)
+def test_weights_far_below_the_largest(dtype, kept, dim, group, depth):
+    """One key takes the weight and its value is 0, so that the output is made of the weights that are 8 to 160 bits
+    smaller: each has to count with its 16 bits, however small, and some that nobody sees are NaN."""
+    sm_scale, lens, news = 0.97 * math.log(2.0), [40, 1500], [2, 1]
+    gen, table, values, caches, scales = _make(lens, 16, 1, dim, dtype, kept, sum(depth))
+    k, v = [x.float() for x in values]
+    k[..., 0] = -torch.tensor(depth, dtype=torch.float32)[torch.randint(2, k.shape[:-1], generator=gen)]
+    v = (1.0 + 0.25 * _normal(gen, *v.shape)).clamp(0.25, 1.75) * (100.0 if kept is E4 else 8192.0)
+    for z in range(2):
+        k[table[z][0], 3, 0, 0] = 0.0
+        v[table[z][0], 3] = 0.0
+    k, v = k.to(kept), v.to(kept)
+    if kept is E4:
+        scales = [torch.ones(1), torch.full((1,), 81.92)]
+    hidden = v.clone()  # the newest token of request 0 is hidden from the one before
+    hidden.view(torch.uint8 if kept is E4 else torch.int16)[table[0][39 // 16], 39 % 16, 0, dim // 2] = 0x7F if kept is E4 else 0x7FFF
+    # Only the first dimension of a query counts, so that scores are products without a sum; four sizes of them.
+    q = torch.zeros(3, group, dim, dtype=dtype)
+    q[:, :, 0] = torch.tensor([1.0, 0.5, 2.0, 1.0]).repeat(-(-group // 4))[:group].to(dtype)
+    starts, args = [0, 2, 3], (table, lens, sm_scale, [0, 2, 3], True, 0, *scales)
+    want, want_lse = R.attention(q, k, v, *args)[:2]
+    # An exponent of up to X bits: sm_scale, log2 e, their product, the key's scale and the difference from the reference
+    # are rounded to 2^-24 each: 5 X ln 2 2^-24 in the weight.  exp2 and the factors of rescaling and joining: 2^-19.
+    # The weight in the product: 2^-16.  Sums of n terms: n 2^-23 in numerator and denominator.
+    X = 2 * depth[1] * 0.97
+    rel = 5 * X * math.log(2.0) * 2.0 ** -24 + 2.0 ** -19 + 2.0 ** -16 + (max(lens) + 64) * 2.0 ** -23
+    # A weight below 2^-126, the least normal number of 32 bits, counts as 0: each of n misses at most 2^-126 |v| of a sum
+    # that is 1 or more.
+    bound = want.abs() * rel + max(lens) * 2.0 ** -126 * float(v.float().max()) * (81.92 if kept is E4 else 1.0)  # values are not negative
+    fi = torch.finfo(dtype)
+    bound = bound + fi.eps / 2 * (want.abs() + bound) + fi.smallest_normal * fi.eps / 2
+    word = torch.uint8 if kept is E4 else torch.int16
+    for num_sms in (0, 1):
+        for values_seen, last in ((v, 3), (hidden, 1)):
+            lse = torch.empty(3, group, device="cuda")
+            caches[0].view(word).copy_(k.view(word))
+            caches[1].view(word).copy_(values_seen.view(word))
+            out = paged_attention(q.cuda(), *caches, ints(table), ints(lens), sm_scale, starts=ints(starts), num_sms=num_sms,
+                                  k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse).cpu().double()
+            rows = [0, 1, 2] if last == 3 else [0, 2]
+            off = float(((out - want).abs() - bound)[rows].max())
+            assert off <= 0, f"out off by {off} over its bound, {float(((out - want).abs() / want.abs())[rows].max())} of it"
+            assert float((lse.cpu().double() - want_lse).abs().max()) <= 2.0 ** -19 + max(lens) * 2.0 ** -24
