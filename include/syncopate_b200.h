@@ -504,7 +504,9 @@ int syn_page_plan(const syn_page_plan_args* args, void* stream);
 
 /* Appends the keys and values of a step to the cache: row t of k and v [tokens, Hkv, D] goes to slot
  * slots[t] of k_cache and v_cache [num_pages, page_size, Hkv, D] (one layout for both caches).  A
- * negative slot is skipped; the slots of a call must differ from one another.  16-bit rows are copied;
+ * negative slot is skipped; the slots of a call must differ from one another.  With `num_slots` above
+ * `tokens` the entries of slots up to there belong to the step: those behind the rows have to be negative, and one that
+ * is not, a token whose key and value nobody gave, is told in `status`.  16-bit rows are copied;
  * with cache_dtype SYN_CACHE_E4M3 the cache holds e4m3(x / scale[head]): the 32-bit quotient, limited to
  * +-448 and rounded to the nearest, ties to even; NaN stays NaN.  D is a multiple of 16; base addresses
  * and strides are multiples of 16 bytes. */
@@ -526,6 +528,7 @@ typedef struct syn_paged_append_args {
   int32_t page_size, num_pages;
   int32_t dtype, cache_dtype;
   int32_t device;
+  int32_t num_slots;
 } syn_paged_append_args;
 int syn_paged_append(const syn_paged_append_args* args, void* stream);
 

@@ -338,6 +338,7 @@ class PagedAppendArgs(C.Structure):
         ("dtype", C.c_int32),
         ("cache_dtype", C.c_int32),
         ("device", C.c_int32),
+        ("num_slots", C.c_int32),
     ]
 
 

@@ -160,11 +160,14 @@ def paged_append(
     *,
     k_scale: Optional[torch.Tensor] = None,
     v_scale: Optional[torch.Tensor] = None,
+    all_slots: bool = False,
     status=None,
     stream=None,
 ) -> None:
     """Writes row ``t`` of ``k`` and ``v`` ``[tokens, heads, dim]`` to slot ``slots[t]`` of the caches
-    ``[pages, page_size, heads, dim]``; negative slots are skipped, ``slots`` may be longer than the rows.
+    ``[pages, page_size, heads, dim]``; negative slots are skipped, ``slots`` may be longer than the rows.  With
+    ``all_slots`` what lies behind the rows has to be padding: a slot there that is not negative, a token without a
+    row, is told in ``status``.
     The slots of one call must differ from one another: of two rows for one slot parts of both may
     stay.  ``dim`` is a multiple of 16, strides are multiples of 16 bytes, the caches have one layout.
     A ``torch.float8_e4m3fn`` cache keeps ``x / scale[head]`` (float32 division), limited to +-448."""
@@ -187,13 +190,14 @@ def paged_append(
         _refuse(where, "the caches must be on the device of k and v and have their heads and dim")
     if index < 0:
         _refuse(where, "the tensors must be on a CUDA device")
-    if tokens == 0:
+    num_slots = slots.numel() if all_slots else tokens
+    if num_slots == 0:
         return
     cs = k_cache.stride()
     args = L.pack_paged_append(
         k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp,
         _check_status(where, index, status), ks[0], ks[1], vs[0], vs[1], cs[0], cs[1], cs[2], tokens, heads, dim, page, pages,
-        _DTYPES[k.dtype], code, index)
+        _DTYPES[k.dtype], code, index, num_slots)
     rc = L.lib().syn_paged_append(args, _stream(index, stream))
     if rc:
         L.check(rc, "syn_paged_append")

@@ -243,6 +243,14 @@ __device__ __forceinline__ uint2 e4m3_quotients(const uint4& v, float scale, flo
 template <typename T, bool E4M3, int TOKENS>
 __global__ void __launch_bounds__(APPEND_THREADS<E4M3>) paged_append_kernel(const __grid_constant__ syn_paged_append_args p) {
   constexpr int THREADS = APPEND_THREADS<E4M3>;
+  // Slots behind the last row, dealt out to the threads of the grid's first column.
+  if (blockIdx.y == 0) {
+    const int64_t skip = static_cast<int64_t>(gridDim.x) * THREADS;
+    for (int64_t t = p.tokens + static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; t < p.num_slots; t += skip) {
+      const int slot = __ldg(p.slots + t);
+      if (slot >= 0) paged_record(p.status, SYN_DEV_BAD_INDEX, static_cast<int>(t), slot);
+    }
+  }
   const int parts = p.D / 8, items = 2 * p.Hkv * parts;
   const int at_once = items < THREADS ? THREADS / items : 1;  // tokens that a block moves side by side
   const int width = items < THREADS ? items : THREADS;
@@ -300,7 +308,8 @@ static int launch_append(const syn_paged_append_args& a, cudaStream_t stream) {
   const int64_t rows = (a.tokens + at_once - 1) / at_once;
   const dim3 one(static_cast<unsigned>(rows), columns), four(static_cast<unsigned>((rows + 3) / 4), columns);
   if (columns > 65535) return SYN_ERR_TOO_LARGE;
-  if (rows * columns >= 4096) paged_append_kernel<T, E4M3, 4><<<four, THREADS, 0, stream>>>(a);
+  if (rows == 0) paged_append_kernel<T, E4M3, 1><<<1, THREADS, 0, stream>>>(a);
+  else if (rows * columns >= 4096) paged_append_kernel<T, E4M3, 4><<<four, THREADS, 0, stream>>>(a);
   else paged_append_kernel<T, E4M3, 1><<<one, THREADS, 0, stream>>>(a);
   SYN_CUDA_TRY(cudaGetLastError());
   return SYN_OK;
@@ -376,17 +385,18 @@ extern "C" int syn_page_plan(const syn_page_plan_args* a, void* stream) {
 
 extern "C" int syn_paged_append(const syn_paged_append_args* a, void* stream) {
   using namespace syn;
-  if (a == nullptr || a->tokens < 0 || a->Hkv <= 0 || a->D <= 0 || a->page_size <= 0 || a->num_pages <= 0)
+  if (a == nullptr || a->tokens < 0 || a->num_slots < 0 || a->Hkv <= 0 || a->D <= 0 || a->page_size <= 0 || a->num_pages <= 0)
     return SYN_ERR_INVALID;
   if (a->dtype != SYN_DTYPE_F16 && a->dtype != SYN_DTYPE_BF16) return SYN_ERR_UNSUPPORTED;
   if (a->cache_dtype != SYN_CACHE_SAME && a->cache_dtype != SYN_CACHE_E4M3) return SYN_ERR_UNSUPPORTED;
   if (a->D % 16 != 0) return SYN_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a->num_pages) * a->page_size > INT_MAX) return SYN_ERR_TOO_LARGE;
   if (static_cast<int64_t>(a->Hkv) * a->D > INT_MAX / 2) return SYN_ERR_TOO_LARGE;
-  if (a->tokens == 0) return SYN_OK;
   syn_paged_append_args p = *a;
+  if (a->status == nullptr) p.num_slots = 0;  // nobody to tell
+  if (a->tokens == 0 && p.num_slots == 0) return SYN_OK;
   const bool e4m3 = a->cache_dtype == SYN_CACHE_E4M3;
-  if (a->k == nullptr || a->v == nullptr || a->slots == nullptr || a->k_cache == nullptr || a->v_cache == nullptr)
+  if ((a->tokens > 0 && (a->k == nullptr || a->v == nullptr)) || a->slots == nullptr || a->k_cache == nullptr || a->v_cache == nullptr)
     return SYN_ERR_INVALID;
   if (e4m3 && (a->k_scale == nullptr || a->v_scale == nullptr)) return SYN_ERR_INVALID;
   if (!paged_aligned(a->k) || !paged_aligned(a->v) || !paged_aligned(a->k_cache) || !paged_aligned(a->v_cache) ||

@@ -913,9 +913,9 @@ class PagedKVCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0, stream=None) -> None:
         """Writes the step's keys and values ``[tokens, kv_heads, head_dim]``.  Rows behind the step's last
-        token are padding and are not written."""
+        token are padding and are not written; fewer rows than the step has tokens are told by :meth:`check`."""
         paged_append(k, v, self.slots, self._k[layer], self._v[layer], k_scale=self.k_scale[layer],
-                     v_scale=self.v_scale[layer], status=self.status, stream=stream)
+                     v_scale=self.v_scale[layer], all_slots=True, status=self.status, stream=stream)
 
     def attend(self, q: torch.Tensor, layer: int = 0, *, sm_scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:

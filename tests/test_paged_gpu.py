@@ -695,3 +695,36 @@ def test_weights_far_below_the_largest(dtype, kept, dim, group, depth):
             off = float(((out - want).abs() - bound)[rows].max())
             assert off <= 0, f"out off by {off} over its bound, {float(((out - want).abs() / want.abs())[rows].max())} of it"
             assert float((lse.cpu().double() - want_lse).abs().max()) <= 2.0 ** -19 + max(lens) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kept", [BF, E4])
+@pytest.mark.parametrize("rows", [0, 1, 3, 700])
+def test_paged_append_records_tokens_without_a_row(kept, rows):
+    gen = torch.Generator().manual_seed(rows)
+    x = _normal(gen, rows, 2, 64, dtype=BF).cuda()
+    scales = dict(k_scale=torch.ones(2, device="cuda"), v_scale=torch.ones(2, device="cuda")) if kept is E4 else {}
+    slots = list(range(rows)) + [-1] * 900
+    caches = [torch.zeros(100, 16, 2, 64, device="cuda").to(kept) for _ in range(2)]
+    for live in (None, rows, rows + 899):
+        at = list(slots)
+        if live is not None:
+            at[live] = 1599
+        status = ints([0] * 4)
+        paged_append(x, x, ints(at), *caches, **scales, all_slots=True, status=status)
+        assert status.tolist()[:3] == ([0, 0, 0] if live is None else [5, live, 1599])
+        for c in caches:
+            flat = c.float().view(-1, 2, 64)
+            assert torch.equal(flat[:rows], x.to(kept).float()) and (flat[rows:] == 0).all()
+
+
+def test_a_step_with_fewer_rows_than_it_planned_is_told():
+    cache = PagedKVCache(8, 16, 1, 64, 2, 64, 40, dtype=HF)
+    x = torch.randn(40, 1, 64, device="cuda").to(HF)
+    cache.plan(ints([20, 1]))
+    cache.append(x[:21], x[:21])
+    cache.check()
+    cache.plan(ints([1, 1]))
+    cache.append(x[:1], x[:1])
+    with pytest.raises(L.SynError) as e:
+        cache.check()
+    assert e.value.code == L.SYN_ERR_BAD_INDEX
