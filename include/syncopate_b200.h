@@ -542,7 +542,8 @@ int syn_paged_append(const syn_paged_append_args* args, void* stream);
  * whatever they hold.  Rows outside all requests are left as they were.  A request with rows behind the end of q is
  * told in `status`; its rows before the end stay in their places.  A row that should see a key behind its row of the
  * table (or from key 2^31 - 64 - page_size on), or on a page outside [0, num_pages), comes out as NaN (and in `status`).
- * Base addresses and strides (in bytes) are multiples of 16.
+ * o and lse share no memory with one another or with what is read.  Base addresses and strides (in bytes) are multiples
+ * of 16.
  * `workspace`: syn_paged_attention_workspace bytes, 16-byte aligned, any contents; it belongs to the call
  * until the call has ended on the GPU. */
 typedef struct syn_paged_attn_args {

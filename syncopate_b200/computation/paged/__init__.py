@@ -95,6 +95,24 @@ def _check_cache(where: str, k_cache, v_cache, dtype, k_scale, v_scale):
     return L.SYN_CACHE_E4M3, k_scale.data_ptr(), v_scale.data_ptr()
 
 
+def _interleaved(a, b) -> bool:
+    """Whether two tensors of one type and shape whose bytes span each other's have no element in common because they
+    lie between one another, token by token or head by head, as columns of one projection do."""
+    size, shape, sa, sb = a.element_size(), a.shape, a.stride(), b.stride()
+    apart, rest = divmod(b.data_ptr() - a.data_ptr(), size)
+    if rest:
+        return False
+    for axis in (0, 1):
+        step = sa[axis]
+        # All coarser steps are multiples of this one: then what lies within a step decides.
+        if step <= 0 or sb[axis] != step or (axis == 1 and shape[0] > 1 and (sa[0] % step or sb[0] % step)):
+            continue
+        inner_a, inner_b = (1 + sum((n - 1) * s for n, s in zip(shape[axis + 1:], st[axis + 1:])) for st in (sa, sb))
+        if apart % step >= inner_a and apart % step + inner_b <= step:
+            return True
+    return False
+
+
 def page_plan(
     lens: torch.Tensor,
     add: torch.Tensor,
@@ -239,7 +257,8 @@ def paged_attention(
     ``table[z]``.  A row at position ``p`` sees the keys ``j <= p`` (``causal=False``: all of the request's),
     with ``window > 0`` those with ``j > p - window`` only.  ``dim`` is 64, 128 or 256; ``q_heads`` a multiple
     of the caches' heads; the caches hold the type of ``q``, or ``torch.float8_e4m3fn`` with ``k_scale`` and
-    ``v_scale`` (what is stored counts times the head's scale).
+    ``v_scale`` (what is stored counts times the head's scale).  ``out`` and ``lse`` share no memory with what is
+    read; views that lie between the rows or heads of ``q`` (columns of one buffer) are fine.
 
     ``lse`` ``[tokens, q_heads]`` (float32, optional) receives the log2-sum-exp, with which results over
     parts of a sequence can be joined.  A row that sees no key gives 0 and -inf.  Keys and values that a row
@@ -285,11 +304,30 @@ def paged_attention(
     if out is not None:
         if out.dtype is not dtype or out.shape != q.shape or out.get_device() != index or out.stride(2) != 1:
             _refuse(where, "out must have the shape, type and device of q and a contiguous head dimension")
-        if out.data_ptr() == q.data_ptr() and tokens:
-            _refuse(where, "out must not overlap q")
     if lse is not None and (lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != q.shape[:2]
                             or not lse.is_contiguous()):
         _refuse(where, "lse must be a contiguous float32 [tokens, q_heads] tensor on the device of q")
+    # Warps write rows while others read theirs: what is written may share no byte with what is read.
+    cs = k_cache.stride()
+    if tokens and (out is not None or lse is not None):
+        q_from, k_from, v_from = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        q_to = q_from + 2 * ((tokens - 1) * qs[0] + (q_heads - 1) * qs[1] + dim)
+        held = ((pages - 1) * cs[0] + (page - 1) * cs[1] + (heads - 1) * cs[2] + dim) * (1 if code else 2) if pages and page else 0
+        o_from = o_to = 0
+        if out is not None:
+            os_ = out.stride()
+            o_from = out.data_ptr()
+            o_to = o_from + 2 * ((tokens - 1) * os_[0] + (q_heads - 1) * os_[1] + dim)
+            if q_from < o_to and o_from < q_to and not _interleaved(q, out):
+                _refuse(where, "out must not overlap q")
+            if k_from < o_to and o_from < k_from + held or v_from < o_to and o_from < v_from + held:
+                _refuse(where, "out must not overlap the caches")
+        if lse is not None:
+            l_from = lse.data_ptr()
+            l_to = l_from + 4 * tokens * q_heads
+            if (q_from < l_to and l_from < q_to or o_from < l_to and l_from < o_to or k_from < l_to and l_from < k_from + held
+                    or v_from < l_to and l_from < v_from + held):
+                _refuse(where, "lse must not overlap q, out or the caches")
     if index < 0:
         _refuse(where, "the tensors must be on a CUDA device")
     if stream is not None:
@@ -303,7 +341,6 @@ def paged_attention(
     if tokens == 0 or requests == 0:
         return out
     os_ = out.stride()
-    cs = k_cache.stride()
     workspace, size = _workspace(q.device, index, num_sms, dim)
     args = L.pack_paged_attn(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),

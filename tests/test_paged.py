@@ -2,6 +2,7 @@
 packed arguments have the layout of the C structs."""
 import ctypes as C
 import os
+import random
 import shutil
 import subprocess
 
@@ -10,7 +11,7 @@ import torch
 
 import paged_ref as R
 from syncopate_b200 import _lib as L
-from syncopate_b200.computation.paged import page_plan, paged_append, paged_attention
+from syncopate_b200.computation.paged import _interleaved, page_plan, paged_append, paged_attention
 from syncopate_b200.operators import PagedKVCache
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -196,3 +197,68 @@ def test_the_reference_plan_by_hand():
     assert (slots, positions) == ([5 * 4 + 3, 3 * 4, 7 * 4, -1, -1], [3, 4, 4, 0, 0])
     assert (starts, lens, top, free) == ([0, 2, 2, 3], [5, 0, 5], 3, [0, 1, 4])
     assert [r[:2] for r in table] == [[5, 3], [7, 3], [2, 7]]
+
+
+def _overlaps(name):
+    """Arguments of paged_attention whose output shares memory with what is read."""
+    args = _attend_tensors()
+    T, H, D = 6, 4, 64
+    args.update(table=torch.zeros(T, 2, **I32), lens=torch.zeros(T, **I32))
+    flat = torch.zeros(64 * 1024, dtype=BF)
+    wide = flat[: T * 3 * H * D].view(T, 3 * H, D)
+    if name == "one head on":
+        args.update(q=wide[:, 1: 1 + H], out=wide[:, 2: 2 + H])
+    elif name == "one token on":
+        args.update(q=flat[: T * H * D].view(T, H, D), out=flat[H * D: (T + 1) * H * D].view(T, H, D))
+    elif name == "half a head on":
+        args.update(q=flat[: T * H * D].view(T, H, D), out=flat[32: 32 + T * H * D].view(T, H, D))
+    elif name == "other strides":
+        args.update(q=wide[:, :H], out=flat[H * D: (T + 1) * H * D].view(T, H, D))
+    elif name == "around the end of a row":  # its last heads lie on the next token's first ones
+        args.update(q=wide[:, :H], out=flat[10 * D: 10 * D + T * 3 * H * D].view(T, 3 * H, D)[:, :H])
+    elif name == "every other head":
+        args.update(q=wide[:, 0: 2 * H: 2], out=wide[:, 2: 2 + 2 * H: 2])
+    elif name in ("out on k_cache", "out on v_cache"):
+        args.update(q=wide[:, :H], out=args[name[7:]].view(-1)[: T * H * D].view(T, H, D))
+    elif name.startswith("lse"):
+        args.update(q=flat[: T * H * D].view(T, H, D), out=flat[T * H * D: 2 * T * H * D].view(T, H, D))
+        args["lse"] = args[name[7:]].reshape(-1)[-2 * T * H:].view(torch.float32).view(T, H)
+    return args
+
+
+@pytest.mark.parametrize("name", ["one head on", "one token on", "half a head on", "other strides", "around the end of a row",
+                                  "every other head", "out on k_cache", "out on v_cache", "lse on q", "lse on out", "lse on k_cache",
+                                  "lse on v_cache"])
+def test_paged_attention_refuses_outputs_over_what_is_read(name):
+    with pytest.raises(ValueError, match="must not overlap"):
+        paged_attention(**_overlaps(name))
+
+
+def test_paged_attention_takes_outputs_between_the_rows_of_its_input():
+    # Refused for want of a GPU alone.
+    T, H, D = 6, 4, 64
+    flat = torch.zeros(64 * 1024, dtype=BF)
+    wide = flat[: T * 3 * H * D].view(T, 3 * H, D)
+    args = {**_attend_tensors(), "table": torch.zeros(T, 2, **I32), "lens": torch.zeros(T, **I32)}
+    for q, out in [(wide[:, :H], wide[:, H: 2 * H]), (wide[:, H: 2 * H], wide[:, :H]), (wide[:, 2 * H:], wide[:, :H]),
+                   (wide[:, 0: 2 * H: 2], wide[:, 1: 2 * H: 2]), (wide[::2, :H], wide[1::2, :H]),
+                   (flat[: T * H * D].view(T, H, D), flat[T * H * D: 2 * T * H * D].view(T, H, D))]:
+        n = q.shape[0]
+        change = dict(q=q, out=out, table=args["table"][:n], lens=args["lens"][:n])
+        with pytest.raises(ValueError, match="CUDA device"):
+            paged_attention(**{**args, **change})
+
+
+def test_outputs_taken_as_interleaved_share_no_element():
+    rng, taken = random.Random(0), 0
+    for _ in range(4000):
+        shape = tuple(rng.randint(1, 4) for _ in range(3))
+        strides = [(rng.choice([2, 4, 6, 8, 12, 16, 24, 32]), rng.choice([1, 2, 3, 4, 6, 8, 12]), 1) for _ in range(2)]
+        if rng.random() < 0.7:
+            strides[1] = strides[0]
+        buf = torch.arange(400, dtype=torch.int32)
+        a, b = (buf.as_strided(shape, s, rng.randint(0, 40)) for s in strides)
+        if _interleaved(a, b):
+            taken += 1
+            assert not set(a.flatten().tolist()) & set(b.flatten().tolist()), (shape, strides)
+    assert taken > 300
