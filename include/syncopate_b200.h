@@ -537,6 +537,7 @@ int syn_paged_append(const syn_paged_append_args* args, void* stream);
  * tokens of the lens[z] in its cache: row i of n sits at position p = lens[z] - n + i and sees the keys
  * j <= p (`causal`; else all of them) with j > p - window (`window` > 0, causal only).
  *   o = sum_j softmax_j(q . k_j * sm_scale) v_j,  lse [tokens, Hq] (may be NULL) = log2 sum_j exp(...)
+ * Scores are meant to stay below 2^29 in magnitude: 32 bits leave larger ones no place behind the point.
  * Keys and values of an 8-bit cache count as k_scale[head] and v_scale[head] times what is stored.  A row
  * that sees no key gives 0 and lse = -inf; keys and values that a row does not see do not touch it,
  * whatever they hold.  Rows outside all requests are left as they were.  A request with rows behind the end of q is

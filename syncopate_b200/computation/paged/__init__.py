@@ -266,6 +266,7 @@ def paged_attention(
     they were (0 where ``out`` is not given).  A row that should see a key without a valid page is NaN.  A
     request with rows behind the end of ``q`` is told in ``status``; its other rows keep their positions.
 
+    Scores are meant to stay below 2^29 in magnitude (32 bits leave larger ones no place behind the point).
     Sums, the running maximum and the output are held in 32 bits until the one rounding to ``q``'s type.
     Returns ``out``."""
     where = "paged_attention"

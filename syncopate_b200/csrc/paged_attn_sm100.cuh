@@ -20,6 +20,7 @@
 //     in a fixed order (the warps of a block that work on one and the same unit join theirs first): results do
 //     not depend on timing, there are no atomics and no state between calls.
 #pragma once
+#include <float.h>
 #include <math_constants.h>
 
 #include <type_traits>
@@ -768,10 +769,10 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     auto lo = [&](int at) { return paged_seen_from(a, r.len, at); };
     auto hi = [&](int at) { return paged_seen_to(a, r.len, at); };
     // From product to power of two; a key that is not seen gets the product that stands for a power of -inf, so the
-    // factor must not be 0 (which 1e-30 stands for: scores then differ by less than a rounding).
-    float mult = a.sm_scale * CUDART_L2E_F;
-    if constexpr (C::E4M3) mult *= a.k_scale[kv_head];
-    if (fabsf(mult) < 1e-30f) mult = 1e-30f;
+    // factor must not be 0: the least normal number then stands for it.
+    auto nonzero = [](float x) { return fabsf(x) < FLT_MIN ? copysignf(FLT_MIN, x) : x; };
+    const float scale = a.sm_scale * CUDART_L2E_F, key_scale = C::E4M3 ? a.k_scale[kv_head] : 1.f;
+    const float mult = nonzero(scale * key_scale);
     const float unseen = mult > 0.f ? -CUDART_INF_F : CUDART_INF_F;
     const T* qrow[RT];
 #pragma unroll
@@ -802,7 +803,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
         const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
         up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        const float back = copysignf(fmaxf(fabsf(mult) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23), 1e-37f), mult);
+        const float back = nonzero(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * key_scale);
 #pragma unroll
         for (int c = 0; c < 2; ++c) down[2 * i + c] = __shfl_sync(~0u, back, (2 * t4 + c) * 4);
       }

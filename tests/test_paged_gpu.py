@@ -728,3 +728,14 @@ def test_a_step_with_fewer_rows_than_it_planned_is_told():
     with pytest.raises(L.SynError) as e:
         cache.check()
     assert e.value.code == L.SYN_ERR_BAD_INDEX
+
+
+@pytest.mark.parametrize("size, sm_scale", [(1e16, 1e-33), (1e16, -1e-33), (1e18, 1e-37)])
+def test_the_smallest_scales_of_the_scores(size, sm_scale):
+    lens, news = [100, 700], [3, 2]
+    gen, table, values, caches, _ = _make(lens, 16, 2, 128, BF, BF, 43)
+    q, k = (_normal(gen, 5, 8, 128) * size).to(BF), (values[0].float() * size).to(BF)
+    caches[0].copy_(k)
+    lse = torch.empty(5, 8, device="cuda")
+    out = paged_attention(q.cuda(), *caches, ints(table), ints(lens), sm_scale, starts=ints([0, 3, 5]), window=300, lse=lse)
+    _compare(out.cpu(), lse.cpu(), R.attention(q, k, values[1], table, lens, sm_scale, [0, 3, 5], True, 300))
