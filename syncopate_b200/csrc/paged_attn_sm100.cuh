@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
         top = max(top, __shfl_xor_sync(~0u, top, 1));
         top = max(top, __shfl_xor_sync(~0u, top, 2));
         const int e = static_cast<int>(top >> 7);  // biased exponent: the row becomes less than 2^15
-        const int shift = e == 0xFF || top == 0 ? 0 : min(max(141 - e, -100), 100);
+        const int shift = e == 0xFF || top == 0 ? 0 : min(141 - e, 100);  // from -113 on
         up[i] = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
         const float back = nonzero(scale * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * key_scale);
 #pragma unroll

@@ -739,3 +739,13 @@ def test_the_smallest_scales_of_the_scores(size, sm_scale):
     lse = torch.empty(5, 8, device="cuda")
     out = paged_attention(q.cuda(), *caches, ints(table), ints(lens), sm_scale, starts=ints([0, 3, 5]), window=300, lse=lse)
     _compare(out.cpu(), lse.cpu(), R.attention(q, k, values[1], table, lens, sm_scale, [0, 3, 5], True, 300))
+
+
+@pytest.mark.parametrize("power, sm_scale", [(0, 0.09), (100, 0.09 * 2.0 ** -100), (113, 0.09 * 2.0 ** -113), (120, 0.09 * 2.0 ** -120)])
+def test_the_largest_queries_over_an_8_bit_cache(power, sm_scale):
+    lens = [100, 700]
+    gen, table, values, caches, scales = _make(lens, 16, 2, 128, BF, E4, 42)
+    q = (_normal(gen, 2, 8, 128) * 2.0 ** power).to(BF)
+    lse = torch.empty(2, 8, device="cuda")
+    out = paged_attention(q.cuda(), *caches, ints(table), ints(lens), sm_scale, k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse)
+    _compare(out.cpu(), lse.cpu(), R.attention(q, values[0], values[1], table, lens, sm_scale, None, True, 0, *scales))
