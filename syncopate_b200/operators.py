@@ -888,9 +888,10 @@ class PagedKVCache:
             if s is not None and tuple(s.shape) != (layers, kv_heads):
                 raise ValueError(f"scales must be [layers, kv_heads] = [{layers}, {kv_heads}]")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self.page_size, self.dtype, self.device = page_size, dtype, device
+        self.page_size, self.dtype = page_size, dtype
         ints = dict(dtype=torch.int32, device=device)
         self.kv = torch.empty(layers, 2, num_pages, page_size, kv_heads, head_dim, dtype=kept, device=device)
+        self.device = self.kv.device  # with its index, where `device` says no more than "cuda"
         self.k_scale = [None] * layers if k_scale is None else list(k_scale.to(device, torch.float32).contiguous())
         self.v_scale = [None] * layers if v_scale is None else list(v_scale.to(device, torch.float32).contiguous())
         self._k = [self.kv[i, 0] for i in range(layers)]

@@ -749,3 +749,8 @@ def test_the_largest_queries_over_an_8_bit_cache(power, sm_scale):
     lse = torch.empty(2, 8, device="cuda")
     out = paged_attention(q.cuda(), *caches, ints(table), ints(lens), sm_scale, k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse)
     _compare(out.cpu(), lse.cpu(), R.attention(q, values[0], values[1], table, lens, sm_scale, None, True, 0, *scales))
+
+
+def test_the_cache_knows_its_device():
+    cache = PagedKVCache(4, 16, 1, 64, 2, 64, 8, device="cuda")
+    assert cache.device == cache.kv.device == torch.device("cuda", torch.cuda.current_device())
