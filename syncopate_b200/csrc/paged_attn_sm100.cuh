@@ -32,8 +32,12 @@ namespace syn {
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
 // The reference a row's weights are taken against (m) follows its maximum only when that has risen by more
-// than this power of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
+// than PA_SLACK powers of two: a vote without shuffles on most steps, and few rescales.  Weights stay below 2^8.
 constexpr float PA_SLACK = 8.f;
+// Halves hold all bits of numbers from 2^-14 to 2^16, so weights that may enter products of halves are taken against
+// a reference that lies 2^11 below and follows sooner: they stay below 2^15, a row's largest is 2^11 or more, and from
+// PA_SMALL on two halves hold 17 bits.  A step with smaller ones takes the products of PAIR_TF32.
+constexpr float PA_SLACK_HALF = 4.f, PA_BIAS = 11.f, PA_SMALL = 0x1p-8f;
 constexpr float PA_NONE = -1e30f;  // reference of a row without a key so far
 constexpr int PA_DESC = 12;  // int32 words a worker leaves for the join (PagedJoin)
 
@@ -319,29 +323,29 @@ __device__ __forceinline__ void each_v(uint32_t v, int lane, int kk, F f) {
 
 // The weights of an 8-row tile at 16 keys, from the scores' fragment (keys by rows) to the values' products: each as two
 // numbers of fewer bits, the second one what the first left, so that their rounding does not add to that of the output.
-// bf16 values: two bf16 (16 bits).  Halves, 8-bit values among them: two TF32 (20 bits).  Two halves would be twice as fast
-// a product but lose the weights 2^-14 and more below the largest, and where a key takes the weight and its values are
-// small the output is made of those.  What it costs: nothing with 8 rows of 128 16-bit dimensions (113 us), 8-bit caches
-// 0.5 % (D = 64: 70 us -> 77), 32 rows 437 us -> 524 (8 bits 413 -> 468).
-template <bool BF16>
-struct PagedWeights;
-
-template <>
-struct PagedWeights<true> {
+//   bf16 values: two bf16, 16 bits.
+//   Halves, 8-bit values among them: two halves, 17 bits, where no weight of the step is smaller than those hold; else
+//   two TF32, 20 bits of any weight.  Small weights count: where a key takes the weight and its values are small, the
+//   output is made of the others.  All steps in TF32: 96 requests on an 8-bit cache 250 us against 222, drafts in fp16
+//   88 against 82, 32 rows 470 against 376.  Scores that spread by tens of powers of two, nearly all steps in TF32: one
+//   token a request 219 (8 bits) and 118 (fp16) against 217 and 116 for scores that do not, 32 rows 516 against 376.
+enum PagedKind { PAIR_BF16, PAIR_F16, PAIR_TF32 };
+template <PagedKind K>
+struct PagedWeights {
   uint32_t hi[2], lo[2];
   __device__ __forceinline__ void set(const float (&w)[4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t top = pack2<true>(w[2 * h], w[2 * h + 1]);
+      const uint32_t top = pack2<K == PAIR_BF16>(w[2 * h], w[2 * h + 1]);
       hi[h] = transpose8(top);
-      const float2 b = unpack2<true>(top);
-      lo[h] = transpose8(pack2<true>(w[2 * h] - b.x, w[2 * h + 1] - b.y));
+      const float2 b = unpack2<K == PAIR_BF16>(top);
+      lo[h] = transpose8(pack2<K == PAIR_BF16>(w[2 * h] - b.x, w[2 * h + 1] - b.y));
     }
   }
 };
 
 template <>
-struct PagedWeights<false> {
+struct PagedWeights<PAIR_TF32> {
   float hi[2][2], lo[2][2];  // [8 keys each][key 2 t4, 2 t4 + 1] of row g
   __device__ __forceinline__ void set(const float (&w)[4]) {
 #pragma unroll
@@ -359,21 +363,18 @@ struct PagedWeights<false> {
 };
 
 // A fragment of the values (16 dimensions by 16 keys) and its product with weights.
-template <bool BF16>
-struct PagedValues;
-
-template <>
-struct PagedValues<true> {
+template <PagedKind K>
+struct PagedValues {
   const uint32_t (&v)[4];
   __device__ __forceinline__ explicit PagedValues(const uint32_t (&v_)[4]) : v(v_) {}
-  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<true>& w) const {
-    mma16816<true>(c, v, w.hi[0], w.hi[1]);
-    mma16816<true>(c, v, w.lo[0], w.lo[1]);
+  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<K>& w) const {
+    mma16816<K == PAIR_BF16>(c, v, w.hi[0], w.hi[1]);
+    mma16816<K == PAIR_BF16>(c, v, w.lo[0], w.lo[1]);
   }
 };
 
 template <>
-struct PagedValues<false> {
+struct PagedValues<PAIR_TF32> {
   float v[2][4];  // of 8 keys each: the even keys of dimensions g and g + 8, the odd ones (an order that the weights share)
   __device__ __forceinline__ explicit PagedValues(const uint32_t (&u)[4]) {
 #pragma unroll
@@ -382,7 +383,7 @@ struct PagedValues<false> {
       v[h][0] = x.x, v[h][1] = y.x, v[h][2] = x.y, v[h][3] = y.y;
     }
   }
-  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<false>& w) const {
+  __device__ __forceinline__ void times(float (&c)[4], const PagedWeights<PAIR_TF32>& w) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       mma1688_tf32(c, v[h], w.hi[h][0], w.hi[h][1]);
@@ -411,6 +412,7 @@ struct alignas(16) PagedOdd {
 template <typename C>
 __device__ __noinline__ void paged_odd(PagedOdd<C>& x, uint32_t v_at, int base, uint32_t groups, const syn_paged_attn_args& a, int len) {
   constexpr bool MBF16 = std::is_same<typename C::type, __nv_bfloat16>::value && !C::E4M3;
+  constexpr PagedKind K = MBF16 ? PAIR_BF16 : PAIR_TF32;
   const int lane = threadIdx.x & 31, t4 = lane & 3;
 #pragma unroll 1
   for (int kk = 0; kk < C::KEYS / 16; ++kk) {
@@ -421,12 +423,12 @@ __device__ __noinline__ void paged_odd(PagedOdd<C>& x, uint32_t v_at, int base, 
       const int from = paged_seen_from(a, len, at), to = paged_seen_to(a, len, at), key = base + kk * 16 + t4 * 2;
       auto seen = [&](int k) { return (k >= from && k < to ? 0xFFFFu : 0u) | (k + 1 >= from && k + 1 < to ? 0xFFFF0000u : 0u); };
       const uint32_t mask0 = seen(key), mask1 = seen(key + 8);
-      PagedWeights<MBF16> w;
+      PagedWeights<K> w;
       w.set(x.w[kk][j]);
       each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
         const uint32_t u[4] = {v[0] & mask0, v[1] & mask0, v[2] & mask1, v[3] & mask1};
         float c[4] = {0.f, 0.f, 0.f, 0.f};
-        PagedValues<MBF16>(u).times(c, w);
+        PagedValues<K>(u).times(c, w);
         if (t4 == (row >> 1 & 3)) {
           x.o[dt][j][row & 1] += row & 1 ? c[1] : c[0];
           x.o[dt][j][2 + (row & 1)] += row & 1 ? c[3] : c[2];
@@ -556,6 +558,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
   using T = typename C::type;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool MBF16 = BF16 && !C::E4M3;  // type of the matrix products: 8-bit values are halves there
+  constexpr float BIAS = MBF16 ? 0.f : PA_BIAS, RISE = MBF16 ? PA_SLACK : PA_SLACK_HALF + PA_BIAS;
   constexpr int RT = C::RT;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_sum[PA_WARPS], s_rest[PA_WARPS];
@@ -957,7 +960,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) rise |= fmaf(s[n][x >> 1][2 * h + (x & 1)], factor(x), -m[x]) > PA_SLACK;
+          for (int h = 0; h < 2; ++h) rise |= fmaf(s[n][x >> 1][2 * h + (x & 1)], factor(x), -m[x]) > RISE;
       if (__any_sync(~0u, rise)) {
 #pragma unroll
         for (int x = 0; x < 2 * RT; ++x) {
@@ -969,6 +972,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          top -= BIAS;
           if (top > m[x]) {
             const float alpha = ex2(m[x] - top);
             m[x] = top;
@@ -981,6 +985,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
           }
         }
       }
+      bool small = false;  // weights between 0 and PA_SMALL
 #pragma unroll
       for (int x = 0; x < 2 * RT; ++x)
 #pragma unroll
@@ -990,7 +995,9 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
             float& v = s[n][x >> 1][2 * h + (x & 1)];
             v = ex2(fmaf(v, factor(x), -m[x]));
             l[x] += v;
+            if constexpr (!MBF16) small |= __float_as_uint(v) - 1u < __float_as_uint(PA_SMALL) - 1u;
           }
+      if constexpr (!MBF16) small = __any_sync(~0u, small);
       const uint32_t v_at = ready();
       refill(true);
 
@@ -1029,18 +1036,24 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[dt][j][c] = x.o[dt][j][c];
       }
+      auto products = [&](auto kind) {
+        constexpr PagedKind K = decltype(kind)::value;
 #pragma unroll
-      for (int kk = 0; kk < SN; ++kk) {
-        if ((odd >> kk & 1) != 0) continue;
-        PagedWeights<MBF16> w[RT];
+        for (int kk = 0; kk < SN; ++kk) {
+          if ((odd >> kk & 1) != 0) continue;
+          PagedWeights<K> w[RT];
 #pragma unroll
-        for (int j = 0; j < RT; ++j) w[j].set(s[kk][j]);
-        each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
-          const PagedValues<MBF16> x(v);
+          for (int j = 0; j < RT; ++j) w[j].set(s[kk][j]);
+          each_v<C>(v_at, lane, kk, [&](int dt, const uint32_t (&v)[4]) {
+            const PagedValues<K> x(v);
 #pragma unroll
-          for (int j = 0; j < RT; ++j) x.times(o[dt][j], w[j]);
-        });
-      }
+            for (int j = 0; j < RT; ++j) x.times(o[dt][j], w[j]);
+          });
+        }
+      };
+      if constexpr (MBF16) products(std::integral_constant<PagedKind, PAIR_BF16>());
+      else if (!small) products(std::integral_constant<PagedKind, PAIR_F16>());
+      else products(std::integral_constant<PagedKind, PAIR_TF32>());
     }
 
     // ---- the unit, or this worker's part of it, is done
