@@ -266,6 +266,11 @@ def paged_attention(
     they were (0 where ``out`` is not given).  A row that should see a key without a valid page is NaN.  A
     request with rows behind the end of ``q`` is told in ``status``; its other rows keep their positions.
 
+    The kernel is chosen by the rows of ``q`` a request on average, padding and requests without rows included:
+    for decoding pass about as many rows as there are requests (``q[:requests]``), not a buffer for prompts (64
+    requests in 512 rows or more: 1.5 times the time, 2.3 times over an 8-bit cache), and a table of the requests
+    that are running.
+
     Scores are meant to stay below 2^29 in magnitude (32 bits leave larger ones no place behind the point).
     Sums, the running maximum and the output are held in 32 bits until the one rounding to ``q``'s type.
     Returns ``out``."""

@@ -1,7 +1,6 @@
-// What the kernels of the paged key-value cache share: status records, the device of a call, and the
-// rounding of 8-bit caches.
+// What the kernels of the paged key-value cache share: status records, the device of a call, and the checks of
+// addresses and strides.
 #pragma once
-#include <cuda_fp8.h>
 #include <limits.h>
 
 #include <initializer_list>

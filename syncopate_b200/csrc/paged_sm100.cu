@@ -2,6 +2,7 @@
 // compute).
 #include "paged.cuh"
 
+#include <cuda_fp8.h>
 #include <math_constants.h>
 
 #include <atomic>

@@ -921,7 +921,8 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, layer: int = 0, *, sm_scale: Optional[float] = None, window: int = 0,
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """Attention of the step's tokens ``q`` ``[tokens, q_heads, head_dim]`` over their sequences (see
-        ``paged_attention``).  Rows behind the step's last token are left as they were."""
+        ``paged_attention``).  Rows behind the step's last token are left as they were, but many of them cost time: a
+        step that is captured for decoding alone is best captured with ``q[:max_requests]``."""
         return paged_attention(q, self._k[layer], self._v[layer], self.table, self.lens,
                                q.shape[-1] ** -0.5 if sm_scale is None else sm_scale, starts=self.starts, window=window,
                                k_scale=self.k_scale[layer], v_scale=self.v_scale[layer], out=out, lse=lse,
