@@ -262,7 +262,8 @@ def paged_attention(
 
     ``lse`` ``[tokens, q_heads]`` (float32, optional) receives the log2-sum-exp, with which results over
     parts of a sequence can be joined.  A row that sees no key gives 0 and -inf.  Keys and values that a row
-    does not see do not touch it, NaN and infinities included.  Rows behind the last request are left as
+    does not see do not touch it, NaN and infinities included; a value that is not finite and seen leaves its
+    dimension not finite (NaN for an infinity too).  Rows behind the last request are left as
     they were (0 where ``out`` is not given).  A row that should see a key without a valid page is NaN.  A
     request with rows behind the end of ``q`` is told in ``status``; its other rows keep their positions.
 
@@ -272,7 +273,8 @@ def paged_attention(
     that are running.
 
     Scores are meant to stay below 2^29 in magnitude (32 bits leave larger ones no place behind the point).
-    Sums, the running maximum and the output are held in 32 bits until the one rounding to ``q``'s type.
+    Sums, the running maximum and the output are held in 32 bits until the one rounding to ``q``'s type; the
+    weights keep 16 bits or more, however small they are, when they meet the values.
     Returns ``out``."""
     where = "paged_attention"
     dtype = q.dtype

@@ -754,3 +754,12 @@ def test_the_largest_queries_over_an_8_bit_cache(power, sm_scale):
 def test_the_cache_knows_its_device():
     cache = PagedKVCache(4, 16, 1, 64, 2, 64, 8, device="cuda")
     assert cache.device == cache.kv.device == torch.device("cuda", torch.cuda.current_device())
+
+
+@pytest.mark.parametrize("dtype, kept", [(BF, BF), (HF, HF), (BF, E4), (HF, E4)])
+@pytest.mark.parametrize("dim, q_heads, heads", [(64, 8, 4), (128, 6, 2), (128, 32, 1), (256, 16, 1)])
+def test_scores_that_spread_over_many_powers_of_two(dtype, kept, dim, q_heads, heads):
+    # Scores of 10 and more on either side: most steps hold weights that halves have no place for.
+    _check_attention([2000, 1, 333, 0, 64], None, q_heads, heads, dim, 16, dtype, kept, seed=51, sm_scale=6.0 * dim ** -0.5, poison=True)
+    _check_attention([2000, 700, 90], [3, 9, 2], q_heads, heads, dim, 16, dtype, kept, seed=52, sm_scale=6.0 * dim ** -0.5, window=450,
+                     num_sms=1, poison=True)
