@@ -403,7 +403,7 @@ __device__ __forceinline__ int paged_seen_to(const syn_paged_attn_args& a, int l
 // Values that are not finite, at keys that only some rows see.  Zero times infinity: they may only enter the rows that see
 // them, so these groups of 16 keys (set in `groups`, the step's first key is `base`) are taken one row at a time, with what
 // it does not see taken out.  A function of its own, whose operands go through memory: inlined, its registers cost the steps
-// without such values (32 rows, 8-bit cache: 624 us against 468).
+// without such values (32 rows, 8-bit cache, all steps in TF32: 624 us against 468).
 template <typename C>
 struct alignas(16) PagedOdd {
   float o[C::DT][C::RT][4], w[C::KEYS / 16][C::RT][4];
