@@ -760,6 +760,7 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
     const int rows = min(C::ROWS, r.n * group - row0);
     const int pos0 = r.pos0;
     const bool one = r.n == 1;  // one new token: spares the divisions
+    const bool newest = one && pos0 >= r.len - 1;  // its only row sees whatever is loaded (behind the end: zeros)
     const int steps = static_cast<int>(min(static_cast<long long>(r.steps - cur.step), t1 - t));
     // This lane's rows: the scores' columns 8 i + 2 t4 + (0, 1) (statistics and output), and 8 i + g (queries).
     // Rows behind the last repeat it.
@@ -1002,8 +1003,8 @@ __global__ void __launch_bounds__(PA_THREADS, C::BLOCKS) paged_attn_kernel(const
       refill(true);
 
       // ---- values, transposed: 16 dimensions by 8 rows a product
-      uint32_t odd = 0;  // groups of 16 keys with values that are not finite, where not every row sees every key
-      if (!whole && r.n > 1) {
+      uint32_t odd = 0;  // groups of 16 keys with values that are not finite, where some row does not see some key
+      if (!whole && !newest) {
         constexpr uint32_t EXP = MBF16 ? 0x7F807F80u : 0x7C007C00u, ONE = MBF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
         for (int kk = 0; kk < SN; ++kk) {

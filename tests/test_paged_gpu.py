@@ -763,3 +763,21 @@ def test_scores_that_spread_over_many_powers_of_two(dtype, kept, dim, q_heads, h
     _check_attention([2000, 1, 333, 0, 64], None, q_heads, heads, dim, 16, dtype, kept, seed=51, sm_scale=6.0 * dim ** -0.5, poison=True)
     _check_attention([2000, 700, 90], [3, 9, 2], q_heads, heads, dim, 16, dtype, kept, seed=52, sm_scale=6.0 * dim ** -0.5, window=450,
                      num_sms=1, poison=True)
+
+
+@pytest.mark.parametrize("dtype, kept", [(BF, BF), (HF, HF), (BF, E4)])
+@pytest.mark.parametrize("rows", [1, 2, 4])
+@pytest.mark.parametrize("window", [0, 6])
+def test_rows_that_are_left_of_a_request_do_not_see_its_newer_tokens(dtype, kept, rows, window):
+    # Five new tokens, of which q has the first few; what only the others see is NaN.
+    length, heads, q_heads, dim = 53, 2, 8, 64
+    gen, table, values, caches, scales = _make([length], 16, heads, dim, dtype, kept, 61)
+    q = _normal(gen, 5, q_heads, dim, dtype=dtype)
+    want = R.attention(q, values[0], values[1], table, [length], 0.1, [0, 5], True, window, *scales)
+    for c in caches:
+        for j in range(length - 5 + rows, length):
+            c[table[0][j // 16], j % 16] = torch.full((heads, dim), math.nan).to(kept)
+    lse = torch.empty(rows, q_heads, device="cuda")
+    out = paged_attention(q[:rows].cuda(), *caches, ints(table), ints([length]), 0.1, starts=ints([0, 5]), window=window,
+                          k_scale=_cuda(scales[0]), v_scale=_cuda(scales[1]), lse=lse)
+    _compare(out.cpu(), lse.cpu(), [w[:rows] for w in want])
